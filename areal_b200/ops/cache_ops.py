@@ -1,0 +1,292 @@
+"""Paged key/value cache in 8 bits: rows quantised into it, attention of single tokens over it, and copies of pages of either
+cache.
+
+Layout of one layer (:class:`QuantPages`): codes e4m3 ``[pages, Hkv, page_size, D]``, fp32 scales ``[pages, Hkv]``, powers of two, one
+for the tokens of a page and head; value = code * scale. The scale of a page that receives rows is the smallest power of two that
+holds its largest finite element (|x| <= 448 * scale), never smaller than what the page already has; where it grows, the page's other
+codes are rounded again to the new one. Writing slot 0 starts a page: what stood in it counts for nothing.
+
+As in :mod:`.functional`, CUDA tensors run the sm_100a kernels and CPU tensors the plain statements (``*_ref``), computed in 64 bits.
+The engine takes this cache with ``NativeInferConfig.kv_cache_dtype = "float8_e4m3"``.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import lib as _lib
+
+F8 = torch.float8_e4m3fn
+KV8_MAX = 448.0
+KV8_E_MIN, KV8_E_MAX = -100, 120
+PAGE_SIZES = (16, 32, 64, 128)
+
+_V, _I, _F, _L = _lib.c_void_p, _lib.c_int, _lib.c_float, _lib.c_ll
+
+
+@dataclass
+class QuantPages:
+    """The 8-bit pages of one layer."""
+
+    k: torch.Tensor              # [pages, Hkv, page_size, D] e4m3
+    v: torch.Tensor
+    k_scale: torch.Tensor        # [pages, Hkv] fp32
+    v_scale: torch.Tensor
+
+    @staticmethod
+    def empty(pages: int, kv_heads: int, page_size: int, dim: int, device) -> "QuantPages":
+        k, v = (torch.zeros(pages, kv_heads, page_size, dim, device=device, dtype=torch.uint8).view(F8) for _ in range(2))
+        ks, vs = (torch.zeros(pages, kv_heads, device=device) for _ in range(2))
+        return QuantPages(k, v, ks, vs)
+
+    def dense(self, dtype=torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values as numbers."""
+        return tuple(c.to(dtype) * s.to(dtype)[:, :, None, None] for c, s in ((self.k, self.k_scale), (self.v, self.v_scale)))
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _check_pages(p: QuantPages, dim: int, dev) -> None:
+    s = p.k.shape
+    _need(p.k.dtype == F8 and p.v.dtype == F8 and len(s) == 4 and p.v.shape == s, "codes: two e4m3 tensors [pages, Hkv, page_size, D]")
+    _need(p.k.is_contiguous() and p.v.is_contiguous(), "codes have to be contiguous")
+    _need(p.k_scale.dtype == torch.float32 and p.v_scale.dtype == torch.float32 and p.k_scale.shape == s[:2] and p.v_scale.shape == s[:2]
+          and p.k_scale.is_contiguous() and p.v_scale.is_contiguous(), "scales: two contiguous fp32 tensors [pages, Hkv]")
+    _need(s[3] == dim and dim in (64, 128), f"head size {dim} with a cache of {s[3]}: 64 or 128 are built")
+    _need(s[2] in PAGE_SIZES, f"page size {s[2]}: one of {PAGE_SIZES}")
+    _need(s[0] > 0 and s[1] > 0, "a cache without pages or heads")
+    _need(p.k.device == dev and p.v.device == dev and p.k_scale.device == dev and p.v_scale.device == dev, "cache on another device than the rows")
+
+
+def _check_table(table, lens, dev) -> None:
+    _need(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.shape[1] > 0, "page table: contiguous int32 [B, width]")
+    _need(lens.dtype == torch.int32 and lens.is_contiguous() and lens.shape == table.shape[:1], "lengths: contiguous int32 [B]")
+    _need(table.device == dev and lens.device == dev, "page table or lengths on another device")
+
+
+def _launch(t: torch.Tensor, name: str, *args) -> None:
+    """Calls a launcher on the device of ``t`` and its current stream."""
+    dev = t.device
+    if dev.index == torch.cuda.current_device():
+        rc = getattr(_lib.get_lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(_lib.get_lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, name)
+
+
+# ----------------------------------------------------------------------------- append
+def _exponent(amax: torch.Tensor) -> torch.Tensor:
+    m, e = torch.frexp(amax)                                     # amax = m * 2^e, m in [1/2, 1)
+    e = torch.where(m <= KV8_MAX / 512, e - 9, e - 8)
+    return torch.where(amax > 0, e, torch.full_like(e, KV8_E_MIN)).clamp(KV8_E_MIN, KV8_E_MAX)
+
+
+def round_e4m3(x: torch.Tensor) -> torch.Tensor:
+    """The nearest e4m3 value of each element (halves to even, beyond 448 the largest), in the type of ``x``."""
+    a = x.abs().clamp(max=KV8_MAX)
+    e = torch.frexp(a)[1].clamp(min=-5) - 4                      # steps of 2^-3 of the leading power, 2^-9 below 2^-6
+    step = torch.ldexp(torch.ones_like(a), e)
+    return torch.copysign(torch.round(a / step) * step, x)
+
+
+def kv8_append_ref(k, v, pages: QuantPages, page_table, seq_lens, cu_seqlens=None) -> None:
+    """Plain statement of :func:`kv8_append`, page by page in 64 bits."""
+    P, _, ps, _ = pages.k.shape
+    B, width = page_table.shape
+    cu = cu_seqlens.tolist() if cu_seqlens is not None else None
+    for b, end in enumerate(seq_lens.tolist()):
+        lo_row, hi_row = (cu[b], cu[b + 1]) if cu else (b, b + (end > 0))
+        start = end - (hi_row - lo_row)
+        if hi_row <= lo_row:
+            continue
+        _need(start >= 0 and end <= width * ps and hi_row <= k.shape[0], f"sequence {b}: {hi_row - lo_row} rows at the end of {end} tokens do not fit")
+        for j in range(start // ps, (end - 1) // ps + 1):
+            page = int(page_table[b, j])
+            _need(0 <= page < P, f"page {page} of sequence {b} is not in the cache")
+            lo, hi = max(start, j * ps), min(end, (j + 1) * ps)
+            slot = lo - j * ps
+            for x, codes, scales in ((k, pages.k, pages.k_scale), (v, pages.v, pages.v_scale)):
+                rows = x[lo_row + lo - start:lo_row + hi - start].double().transpose(0, 1)          # [Hkv, n, D]
+                old = scales[page].double() if slot else torch.zeros_like(scales[page], dtype=torch.float64)
+                amax = torch.where(torch.isfinite(rows), rows.abs(), torch.zeros_like(rows)).amax((1, 2))
+                s = torch.maximum(old, torch.ldexp(torch.ones_like(amax), _exponent(amax)))
+                ratio = torch.where((old > 0) & (s > old), old / s, torch.ones_like(s))
+                block = round_e4m3(codes[page].double() * ratio[:, None, None])
+                block[:, slot:slot + hi - lo] = round_e4m3(rows / s[:, None, None])
+                codes[page] = block.float().to(F8)
+                scales[page] = s.float()
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq_lens: torch.Tensor,
+               cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    """Quantises rows ``k``, ``v`` ``[rows, Hkv, D]`` bf16 into the pages of their sequences, behind what those hold.
+
+    Without ``cu_seqlens`` row ``b`` is the last token of sequence ``b``, at position ``seq_lens[b] - 1``; a row of length 0 has none. With it
+    sequence ``b`` brings the rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` as its last ones; rows behind ``cu_seqlens[B]`` are left out. Rows
+    may be a part of a wider projection (``k.stride(0)`` a multiple of 8 elements, heads dense). A page that gets rows belongs to one
+    sequence. ``page_table`` ``[B, width]`` int32; entries of a sequence beyond its length are not read. An entry out of the cache, or a
+    length beyond the table, sets the device error word (code 6) and writes nothing for that page."""
+    _need(k.dim() == 3 and k.shape == v.shape and k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16, "keys and values: bf16 [rows, Hkv, D]")
+    dev, (rows, Hkv, D) = k.device, k.shape
+    _need(v.device == dev, "keys and values on different devices")
+    _check_pages(pages, D, dev)
+    _check_table(page_table, seq_lens, dev)
+    B = page_table.shape[0]
+    _need(pages.k.shape[1] == Hkv, f"rows of {Hkv} heads into a cache of {pages.k.shape[1]}")
+    if cu_seqlens is None:
+        _need(rows == B, f"{rows} rows for {B} sequences")
+    else:
+        _need(cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.shape == (B + 1,) and cu_seqlens.device == dev,
+              "cu_seqlens: contiguous int32 [B + 1]")
+    if not k.is_cuda:
+        return kv8_append_ref(k, v, pages, page_table, seq_lens, cu_seqlens)
+    if rows == 0 or B == 0:
+        return
+    ks, vs = k.stride(), v.stride()
+    _need(ks[2] == 1 and vs[2] == 1 and (Hkv == 1 or (ks[1] == D and vs[1] == D)), "heads of a row have to be dense")
+    if rows == 1:
+        ks = vs = (Hkv * D,)
+    kp, vp = k.data_ptr(), v.data_ptr()
+    _need(ks[0] % 8 == 0 and vs[0] % 8 == 0 and (kp | vp) % 16 == 0, "rows have to start on 16 bytes")
+    _launch(k, "ab2_kv8_append", kp, vp, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), page_table.data_ptr(),
+            seq_lens.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), B, rows, Hkv, D, pages.k.shape[2], page_table.shape[1],
+            pages.k.shape[0], ks[0], vs[0])
+
+
+# ----------------------------------------------------------------------------- attention of single tokens
+def kv8_decode_ref(q, pages: QuantPages, page_table, seq_lens, scale: Optional[float] = None) -> torch.Tensor:
+    """Plain statement of :func:`kv8_decode` in 64 bits (returned in 64 bits)."""
+    B, Hq, D = q.shape
+    Hkv, ps = pages.k.shape[1:3]
+    scale = D ** -0.5 if scale is None else scale
+    out = torch.zeros(B, Hq, D, dtype=torch.float64, device=q.device)
+    for b, n in enumerate(seq_lens.tolist()):
+        if n <= 0:
+            continue
+        pg = page_table[b, :-(-n // ps)].long()
+        K, V = ((c.view(torch.uint8)[pg].view(F8).double() * s[pg].double()[:, :, None, None]).transpose(0, 1).reshape(Hkv, -1, D)[:, :n]
+                for c, s in ((pages.k, pages.k_scale), (pages.v, pages.v_scale)))
+        z = torch.einsum("hgd,htd->hgt", q[b].double().view(Hkv, Hq // Hkv, D), K) * scale
+        out[b] = torch.einsum("hgt,htd->hgd", torch.softmax(z, -1), V).reshape(Hq, D)
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(dev: int, *sizes: int) -> int:
+    with torch.cuda.device(dev):
+        return int(_lib.get_lib().ab2_kv8_decode_workspace(*sizes))
+
+
+def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one query token per sequence over its first ``seq_lens[b]`` cached tokens: ``softmax(scale q K^T) V``.
+
+    ``q`` ``[B, Hq, D]`` bf16, heads dense, rows a multiple of 8 elements apart (the query part of a wider projection); ``Hq`` a multiple of the cache's
+    heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous, where given);
+    a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
+    length beyond the table, sets the device error word (code 6); the row's result is not to be used. The workspace is allocated in
+    the call, on the current stream, so calls on several streams and captured graphs do not share one. At most 8192 sequences."""
+    _need(q.dim() == 3 and q.dtype == torch.bfloat16, "queries: bf16 [B, Hq, D]")
+    dev, (B, Hq, D) = q.device, q.shape
+    _check_pages(pages, D, dev)
+    _check_table(page_table, seq_lens, dev)
+    P, Hkv, ps, _ = pages.k.shape
+    width = page_table.shape[1]
+    _need(page_table.shape[0] == B, f"{B} queries for {page_table.shape[0]} sequences")
+    _need(Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads over {Hkv} cached ones")
+    _need(B <= 8192 and width * ps < (1 << 31) - 64, "more than 8192 sequences, or a table wider than 2^31 tokens")
+    if out is not None:
+        _need(out.shape == q.shape and out.dtype == torch.bfloat16 and out.is_contiguous() and out.device == dev, "out: contiguous bf16 like the queries")
+    if not q.is_cuda:
+        o = kv8_decode_ref(q, pages, page_table, seq_lens, scale).to(torch.bfloat16)
+        return o if out is None else out.copy_(o)
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=torch.bfloat16, device=dev)
+    if B == 0:
+        return out
+    st = q.stride()
+    _need(st[2] == 1 and (Hq == 1 or st[1] == D), "heads of a row have to be dense")
+    row = st[0] if B > 1 else Hq * D
+    _need(row % 8 == 0 and q.data_ptr() % 16 == 0, "rows have to start on 16 bytes")
+    ws = torch.empty(_decode_workspace(dev.index, B, Hq, Hkv, D, ps, width), dtype=torch.uint8, device=dev)
+    _launch(q, "ab2_kv8_decode", q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
+            page_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, ps, width, P, D ** -0.5 if scale is None else scale, row)
+    return out
+
+
+# ----------------------------------------------------------------------------- page copies
+def copy_pages_ref(buffers, src, dst, tokens=None) -> None:
+    """Plain statement of :func:`copy_pages`."""
+    for t, page_dim, token_dim in buffers:
+        t = t.view(torch.uint8) if t.dtype == F8 else t
+        for i, (s, d) in enumerate(zip(src, dst)):
+            a, b = t.select(page_dim, int(s)), t.select(page_dim, int(d))
+            if tokens is not None and token_dim is not None:
+                a, b = a.narrow(token_dim - 1, 0, int(tokens[i])), b.narrow(token_dim - 1, 0, int(tokens[i]))
+            b.copy_(a)
+
+
+def copy_pages(buffers: Sequence[tuple], src, dst, tokens=None) -> None:
+    """Copies pages ``src[i]`` to ``dst[i]`` in every buffer, all in one launch (256 pairs each): requests that fork from a prompt's partial last
+    page, or pages that move.
+
+    ``buffers``: up to four ``(tensor, page_dim, token_dim)``. The tensor is contiguous; its dims before ``page_dim`` (layers, keys and values) are copied
+    for every page; ``token_dim`` (behind ``page_dim``) counts the tokens of a page, or is None for what belongs to a page as a whole (scales).
+    ``src``, ``dst``, ``tokens``: host sequences of ints or integer arrays; ``tokens[i]`` leading tokens of page i are copied, the rest of the
+    destination stays as it is (None: whole pages). A source may stand for several destinations; no page may be a destination twice, or source and
+    destination at once."""
+    src, dst = np.asarray(src, np.int32).reshape(-1), np.asarray(dst, np.int32).reshape(-1)
+    n = len(src)
+    _need(len(dst) == n and 0 < len(buffers) <= 4, "one destination for each source, one to four buffers")
+    dev, pages, slots = buffers[0][0].device, None, None
+    desc = []
+    for t, page_dim, token_dim in buffers:
+        shape = t.shape
+        _need(t.device == dev and t.is_contiguous() and t.numel() > 0, "buffers: contiguous, on one device")
+        _need(0 <= page_dim < len(shape) and (token_dim is None or page_dim < token_dim < len(shape)), "no such dims")
+        _need(pages in (None, shape[page_dim]), "buffers of different numbers of pages")
+        pages = shape[page_dim]
+        if token_dim is not None:
+            _need(slots in (None, shape[token_dim]), "buffers of different page sizes")
+            slots = shape[token_dim]
+        st, es = t.stride(), t.element_size()
+        planes = t.numel() // (pages * st[page_dim])
+        whole = st[page_dim] * es
+        if tokens is None or token_dim is None:
+            rows, row, tok = 1, whole, 0
+        else:
+            tok = st[token_dim] * es
+            row = tok * shape[token_dim]
+            rows = whole // row
+        _need(whole < (1 << 31) - (1 << 14), "a page of 2 GB")
+        desc += [t.data_ptr(), whole * pages, whole, row, planes, rows, row, tok, pages, 0]
+    if n == 0:
+        return
+    _need(int(src.min()) >= 0 and int(src.max()) < pages and int(dst.min()) >= 0 and int(dst.max()) < pages, f"pages outside of 0 .. {pages - 1}")
+    to = set(dst.tolist())
+    _need(len(to) == n, "a page is the destination of two copies")
+    _need(to.isdisjoint(src.tolist()), "a page is source and destination")
+    if tokens is not None:
+        tokens = np.asarray(tokens, np.int32).reshape(-1)
+        _need(len(tokens) == n and slots is not None and int(tokens.min()) >= 0 and int(tokens.max()) <= slots, "tokens: 0 to the page size, one for each pair")
+    if not dev.type == "cuda":
+        return copy_pages_ref(buffers, src, dst, tokens)
+    pairs = np.empty((n, 3), np.int32)
+    pairs[:, 0], pairs[:, 1], pairs[:, 2] = src, dst, -1 if tokens is None else tokens
+    flat = (ctypes.c_longlong * len(desc))(*desc)
+    _launch(buffers[0][0], "ab2_copy_pages", ctypes.addressof(flat), len(buffers), pairs.ctypes.data, n)
+
+
+_lib.declare("ab2_kv8_append", [_V] * 9 + [_I] * 7 + [_L, _L, _V])
+_lib.declare("ab2_kv8_decode", [_V] * 9 + [_I] * 7 + [_F, _L, _V])
+_lib.declare("ab2_kv8_decode_workspace", [_I] * 6, _L)
+_lib.declare("ab2_copy_pages", [_V, _I, _V, _I, _V])

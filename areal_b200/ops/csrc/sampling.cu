@@ -1,0 +1,763 @@
+// The next token under temperature, top-k, top-p and min-p, from one given uniform number a row.
+//
+//   order: logits falling, equal ones by index;   w_i = exp((x_i - max) * inv_temp)
+//   top-k: the first k of the order;  top-p: of those, every one before which the sum of w is <= top_p * their total
+//   min-p: w_i >= min_p;  W = sum of the kept w;  token = the lowest index whose running sum (by index) passes u * W
+//   log-prob = ln(w / W); a greedy row takes the first of the order and its log-prob over all tokens
+//
+// A token next to a border (of the nucleus, or of u) must not depend on how a sum was rounded, so weights and sums are 64-bit floats.
+//
+// One thread-block cluster = one row; its blocks hold the row in their shared memory, so that the logits are read from memory once,
+// and exchange maxima, counts, sums through distributed shared memory. Steps: (1) load, maximum; (2) a histogram of max - x
+// in steps of 1/64 nat, by counts, and (top-p only) the exact total; the edges of the bins bound the sums before each bin from both
+// ends, which leaves a bin or two in which the border can lie; (3) everything down to there goes to a list in the first block (a few dozen
+// tokens of a usual row), which sorts it and finishes alone. A nucleus of more than 2048 tokens: only the undecided bins go
+// to the list, the first block gives the last kept value and how many tokens with that value are kept, and the blocks then sum
+// their kept weights by index. Where even the undecided bins are too full (thousands of equal logits), the range is cut again.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace ab2 {
+namespace cg = cooperative_groups;
+
+constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32;
+constexpr int SF_BINS = 2048;          // four for each thread
+constexpr int SF_CAP = 2048;           // entries of the list
+constexpr int SF_SEGS = 128;           // pieces of a block's share with sums of their own, eight for each warp
+constexpr int SF_MAX_CLUSTER = 8;
+constexpr float SF_PER_NAT = 64.f;
+
+struct SampleArgs {
+  const float* logits;
+  long long ld;
+  const float *u, *inv_temp, *top_p, *min_p;
+  const int *top_k, *greedy;           // greedy may be null
+  int* out_tok;
+  float* out_logp;
+  int V, share;                        // share: logits of one block, a multiple of 4
+  int aligned;                         // rows start on 16 bytes
+};
+
+struct SampleShared {
+  unsigned long long list[SF_CAP];
+  unsigned int hist[SF_BINS];
+  double tab[64];                      // 2^(j/64)
+  double seg_sum[SF_SEGS];
+  int seg_tie[SF_SEGS];
+  // what the blocks of the cluster tell one another; two sets in turn, since a fast block may write the next before a slow one has read
+  double pub_sum[2][SF_MAX_CLUSTER], pub_sum2[2][SF_MAX_CLUSTER];
+  float pub_hi[2][SF_MAX_CLUSTER], pub_lo[2][SF_MAX_CLUSTER], pub_hi2[2][SF_MAX_CLUSTER], pub_lo2[2][SF_MAX_CLUSTER];
+  int pub_int[2][SF_MAX_CLUSTER];
+  double red[SF_WARPS], red2[SF_WARPS];
+  float fred[4][SF_WARPS];
+  int ired[SF_WARPS];
+  float thr;
+  int ties, list_n, cut[4];
+};
+
+// exp(d) for d <= 0 in 64 bits: exp(d) = 2^k * 2^(j/64) * exp(r), |r| <= ln 2 / 128, the last by its Taylor polynomial (table-driven
+// exponentials after P. T. P. Tang, 1989; relative error below 5e-14). Zero below e^-700.
+__device__ __forceinline__ double weight(double d, const double* tab) {
+  if (!(d >= -700.0)) return 0.0;
+  const double big = 6755399441055744.0;                       // 1.5 * 2^52: adding it rounds to a whole number
+  const double t = fma(d, 92.332482616893656877, big);         // 64 / ln 2
+  const int k = __double2loint(t);
+  const double r = fma(t - big, -0.010830424696249145, d);     // ln 2 / 64
+  double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  const double w = p * tab[k & 63];
+  return __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
+}
+// Order-preserving map of floats to unsigned.
+__device__ __forceinline__ unsigned int key_of(float x) {
+  const unsigned int b = __float_as_uint(x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float float_of(unsigned int k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int warp_sum_i(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_min(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Sorts list[0 .. n2), n2 a power of two, falling.
+__device__ __forceinline__ void sort_falling(unsigned long long* list, int n2) {
+  for (int k = 2; k <= n2; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = threadIdx.x; i < n2 / 2; i += SF_THREADS) {
+        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+        const unsigned long long x = list[a], y = list[b];
+        if ((x < y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
+      }
+      __syncthreads();
+    }
+}
+__device__ __forceinline__ int pow2_above(int n) {
+  int p = 2;
+  while (p < n) p <<= 1;
+  return p;
+}
+
+// Sum over the block of each thread's value before this thread (exclusive, in thread order), and the total.
+__device__ __forceinline__ double block_scan(double v, double* red, double* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = s;
+  __syncthreads();
+  double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int w = 0; w < SF_WARPS; ++w) {
+    if (w == warp) before = all;
+    all += red[w];
+  }
+  *total = all;
+  return before + (s - v);
+}
+__device__ __forceinline__ int block_scan_i(int v, int* red, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = s;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < SF_WARPS; ++w) {
+    if (w == warp) before = all;
+    all += red[w];
+  }
+  *total = all;
+  return before + s - v;
+}
+
+// The range of values that is being cut into bins: x in [lo, hi], bin = (hi - x) * scale, the last bin open below.
+struct Range {
+  float hi, lo;
+  double scale;
+  bool first;                          // the whole row, 64 bins a nat: single precision is enough
+};
+__device__ __forceinline__ int bin_of(const Range& r, float x) {
+  if (r.first) return (int)fminf((r.hi - x) * (float)r.scale, (float)(SF_BINS - 1));
+  return (int)fmin(((double)r.hi - (double)x) * r.scale, (double)(SF_BINS - 1));
+}
+
+__global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __grid_constant__ SampleArgs a) {
+  extern __shared__ __align__(16) unsigned char dsm[];
+  SampleShared& sh = *reinterpret_cast<SampleShared*>(dsm);
+  float* xs = reinterpret_cast<float*>(dsm + (sizeof(SampleShared) + 15) / 16 * 16);
+  cg::cluster_group cl = cg::this_cluster();
+  const int nb = cl.num_blocks(), me = cl.block_rank();
+  const int row = blockIdx.x / nb, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_trigger();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");          // met below: every block runs before its memory is written from outside
+  const int begin = min(me * a.share, a.V), n = min(a.share, a.V - begin);       // this block's logits
+  int buf = 0;                                                                   // set of the published values in use
+  // ---- the row into shared memory, its maximum
+  float mx = -INFINITY;
+  {
+    const float* src = a.logits + (size_t)row * a.ld + begin;
+    auto clean = [](float x) { return x == x ? x : -INFINITY; };
+    if (a.aligned) {
+      const int n4 = n >> 2;
+#pragma unroll 4
+      for (int i = tid; i < n4; i += SF_THREADS) {
+        float4 v = __ldcs(reinterpret_cast<const float4*>(src) + i);
+        v.x = clean(v.x); v.y = clean(v.y); v.z = clean(v.z); v.w = clean(v.w);
+        reinterpret_cast<float4*>(xs)[i] = v;
+        mx = fmaxf(mx, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+      }
+      for (int i = 4 * n4 + tid; i < n; i += SF_THREADS) { const float v = clean(src[i]); xs[i] = v; mx = fmaxf(mx, v); }
+    } else {
+      for (int i = tid; i < n; i += SF_THREADS) { const float v = clean(src[i]); xs[i] = v; mx = fmaxf(mx, v); }
+    }
+  }
+  for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
+  if (tid < 64) sh.tab[tid] = exp2(tid * (1.0 / 64.0));
+  if (tid == 0) sh.list_n = 0;
+  mx = warp_max(mx);
+  if (lane == 0) sh.fred[0][warp] = mx;
+  __syncthreads();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (tid < nb) {
+    float m = sh.fred[0][0];
+#pragma unroll
+    for (int w = 1; w < SF_WARPS; ++w) m = fmaxf(m, sh.fred[0][w]);
+    cl.map_shared_rank(&sh, tid)->pub_hi[buf][me] = m;
+  }
+  cl.sync();
+  float xmax = -INFINITY;
+  for (int i = 0; i < nb; ++i) xmax = fmaxf(xmax, sh.pub_hi[buf][i]);
+  buf ^= 1;
+  if (xmax == -INFINITY) {                                                       // nothing has any weight
+    if (me == 0 && tid == 0) { a.out_tok[row] = -1; a.out_logp[row] = -INFINITY; }
+    return;
+  }
+  if (xmax == INFINITY) {                                                        // only infinite logits have weight, all the same
+    for (int i = tid; i < n; i += SF_THREADS) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+    xmax = 0.f;
+    __syncthreads();
+  }
+  const float itf = a.inv_temp[row] >= 0.f ? fminf(a.inv_temp[row], 1e30f) : 0.f;
+  const double it = (double)itf, top = (double)xmax;
+  auto w_of = [&](float x) { return x == xmax ? 1.0 : weight(((double)x - top) * it, sh.tab); };
+  const bool greedy = a.greedy && a.greedy[row] != 0;
+  const float tpf = a.top_p[row];
+  const double top_p = (double)fmaxf(tpf, 0.f), min_p = (double)fminf(a.min_p[row], 1.f);
+  const bool by_mass = !greedy && tpf < 1.f;
+  int K = a.top_k[row];
+  if (greedy || K <= 0 || K >= a.V) K = 0;
+  const bool by_min = !greedy && min_p > 0.0;
+
+  // publishes one sum for each block; after the next cluster barrier pub_sum[buf] has them all
+  auto publish_sum = [&](double v) {
+    v = warp_sum_d(v);
+    __syncthreads();
+    if (lane == 0) sh.red[warp] = v;
+    __syncthreads();
+    if (tid < nb) {
+      double s = 0.0;
+#pragma unroll
+      for (int w = 0; w < SF_WARPS; ++w) s += sh.red[w];
+      cl.map_shared_rank(&sh, tid)->pub_sum[buf][me] = s;
+    }
+  };
+  auto all_sum = [&]() {
+    double s = 0.0;
+    for (int i = 0; i < nb; ++i) s += sh.pub_sum[buf][i];
+    return s;
+  };
+
+  if (greedy) {
+    double s = 0.0;
+    int first = 0x7fffffff;
+    for (int i = tid; i < n; i += SF_THREADS) {
+      const float x = xs[i];
+      s += w_of(x);
+      if (x == xmax) first = min(first, begin + i);
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) sh.ired[warp] = first;
+    publish_sum(s);                                                              // its barriers cover ired too
+    if (tid < nb) {
+      int f = sh.ired[0];
+#pragma unroll
+      for (int w = 1; w < SF_WARPS; ++w) f = min(f, sh.ired[w]);
+      cl.map_shared_rank(&sh, tid)->pub_int[buf][me] = f;
+    }
+    cl.sync();
+    if (me == 0 && tid == 0) {
+      int f = 0x7fffffff;
+      for (int i = 0; i < nb; ++i) f = min(f, sh.pub_int[buf][i]);
+      a.out_tok[row] = f;
+      a.out_logp[row] = (float)-log(all_sum());
+    }
+    return;
+  }
+
+  float thr = -INFINITY;                // kept: x > thr, and the first `ties` (by index) of those equal to it
+  int ties = 0;
+  double total = 0.0;                   // what top_p is a share of
+  // by count first (top-k), then by mass (top-p), each only where asked for; min-p alone goes through once to try for the list
+  for (int stage = 0; stage < 2; ++stage) {
+    const bool counting = stage == 0 && K > 0;
+    const bool mass = stage == 1 && by_mass;
+    const bool min_only = stage == 1 && !by_mass && by_min && K == 0;
+    if (!counting && !mass && !min_only) continue;
+    // top-p behind a top-k that was too long for the list: its total is that of the kept ones
+    const bool limited = stage == 1 && K > 0;
+    Range r{xmax, -INFINITY, (double)(itf * SF_PER_NAT), true};
+    double s_above = 0.0;               // exact mass and number of what is certainly kept
+    int c_above = 0;
+    for (int round = 0;; ++round) {
+      // ---- histogram of this range
+      double s = 0.0;
+      const bool sum_now = mass && round == 0;
+      for (int i = tid; i < n; i += SF_THREADS) {
+        const float x = xs[i];
+        if (x == -INFINITY) continue;
+        if (limited && x <= thr) continue;                                        // of those equal to thr `ties` are there: added below
+        if (sum_now) s += w_of(x);
+        if (x <= r.hi && x >= r.lo) atomicAdd(&sh.hist[bin_of(r, x)], 1u);
+      }
+      if (sum_now) publish_sum(s);
+      cl.sync();
+      if (sum_now) {
+        total = all_sum();
+        if (limited) total += ties * w_of(thr);
+        buf ^= 1;
+      }
+      // ---- counts of the cluster, and where the border can be
+      unsigned int c[4] = {0u, 0u, 0u, 0u};
+      for (int i = 0; i < nb; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(cl.map_shared_rank(sh.hist, i))[tid];
+        c[0] += v.x; c[1] += v.y; c[2] += v.z; c[3] += v.w;
+      }
+      if (limited && thr <= r.hi && thr >= r.lo && (bin_of(r, thr) >> 2) == tid) c[bin_of(r, thr) & 3] += ties;
+      const int own = (int)(c[0] + c[1] + c[2] + c[3]);
+      int c_total;
+      const int c_before = block_scan_i(own, sh.ired, &c_total);
+      if (tid == 0) { sh.cut[0] = SF_BINS; sh.cut[1] = SF_BINS; sh.cut[2] = c_total; sh.cut[3] = 0; }
+      __syncthreads();
+      if (counting) {
+        if (round == 0 && c_total < K) { K = 0; break; }                          // fewer than k tokens have any weight
+        int at = c_above + c_before;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (at < K && at + (int)c[j] >= K) { sh.cut[0] = sh.cut[1] = 4 * tid + j; sh.cut[2] = c_before + (at - c_above - c_before) + (int)c[j]; sh.cut[3] = at - c_above; }
+          at += (int)c[j];
+        }
+      } else if (mass) {
+        // weights of bin b lie in w0 * f^b * [f, 1], f the ratio of neighbouring edges, but for the open last bin
+        const double f = exp(-it / r.scale), w0 = exp(((double)r.hi - top) * it) * exp(-it / r.scale * 4.0 * tid);
+        double lo[4], m = 0.0, e = w0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = (4 * tid + j < SF_BINS - 1) ? c[j] * e * f : 0.0;
+          m += lo[j];
+          e *= f;
+        }
+        double m_all;
+        double m_cum = block_scan(m, sh.red, &m_all);
+        if (tid == SF_THREADS - 1) sh.red2[0] = c[3] * (e / f);                   // upper bound of the last bin
+        __syncthreads();
+        const double last_hi = sh.red2[0], slack = 2e-5;
+        const double want = top_p * total - s_above;                              // mass up to the border, of this range
+        const double rest = total - top_p * total;                               // mass behind it
+        // mass behind the last bin of the range (later rounds): total - s_above - what the range holds; only bounded by the head then
+        int at = c_before, b1 = SF_BINS, b2 = SF_BINS, c1 = 0, c2 = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m_cum += lo[j];
+          const double head_hi = m_cum / f * (1.0 + slack), head_lo = m_cum * (1.0 - slack);
+          const double tail_hi = ((m_all - m_cum) / f + last_hi) * (1.0 + slack), tail_lo = (m_all - m_cum) * (1.0 - slack);
+          const bool end = 4 * tid + j == SF_BINS - 1;
+          const bool maybe = c[j] && (end || (head_hi > want && (!r.first || tail_lo < rest)));
+          const bool sure = c[j] && (head_lo > want || (r.first && tail_hi < rest));
+          if (maybe && b1 == SF_BINS) { b1 = 4 * tid + j; c1 = at; }
+          at += (int)c[j];
+          if (sure && b2 == SF_BINS) { b2 = 4 * tid + j; c2 = at; }
+        }
+        if (b1 < SF_BINS) atomicMin(&sh.cut[0], b1);
+        if (b2 < SF_BINS) atomicMin(&sh.cut[1], b2);
+        __syncthreads();
+        if (b1 < SF_BINS && sh.cut[0] == b1) sh.cut[3] = c1;
+        if (b2 < SF_BINS && sh.cut[1] == b2) sh.cut[2] = c2;
+      } else {
+        // min-p: ln(1 / min_p) below the maximum, a bin further for what rounding does to the edges
+        const double t = -log(min(min_p, 1.0)) * (double)SF_PER_NAT + 1.0;
+        const int b2 = t < (double)(SF_BINS - 1) ? (int)t : SF_BINS - 1;
+        if (tid == b2 >> 2) {
+          int at = c_before;
+          for (int j = 0; j <= (b2 & 3); ++j) at += (int)c[j];
+          sh.cut[0] = 0; sh.cut[1] = b2; sh.cut[2] = at; sh.cut[3] = 0;
+        }
+      }
+      __syncthreads();
+      int b1 = sh.cut[0], b2 = sh.cut[1], before = sh.cut[3];
+      const int upto = sh.cut[2];
+      if (b2 >= SF_BINS) b2 = SF_BINS - 1;
+      if (b1 > b2) b1 = before = 0;
+      const bool whole = r.first && upto <= SF_CAP && !limited;
+      const int undecided = upto - before;
+      if (min_only && !whole) break;                                              // every token is looked at anyway
+      const bool listed = whole || undecided <= SF_CAP;
+      // ---- second look: the list, or the mass and range of what is decided
+      s = 0.0;
+      double s_one = 0.0;
+      float hi1 = -INFINITY, lo1 = INFINITY, hi2 = -INFINITY, lo2 = INFINITY;
+      SampleShared* head = cl.map_shared_rank(&sh, 0);
+      for (int i0 = 0; i0 < n; i0 += SF_THREADS) {
+        const int i = i0 + tid;
+        const float x = i < n ? xs[i] : -INFINITY;
+        bool take = false;
+        if (x != -INFINITY && !(limited && x <= thr) && x >= r.lo) {
+          const int b = x > r.hi ? -1 : bin_of(r, x);
+          if (whole) {
+            take = b <= b2;
+          } else {
+            if (b < b1) s += mass && b >= 0 ? w_of(x) : 0.0;                      // those above the range were summed before
+            else if (b <= b2) {
+              if (listed) take = true;
+              else if (b == b1) { s_one += mass ? w_of(x) : 0.0; hi1 = fmaxf(hi1, x); lo1 = fminf(lo1, x); }
+              else { hi2 = fmaxf(hi2, x); lo2 = fminf(lo2, x); }
+            }
+          }
+        }
+        const unsigned int who = __ballot_sync(0xffffffffu, take);
+        if (who) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&sh.list_n, __popc(who));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+          if (take && at < SF_CAP) sh.list[at] = ((unsigned long long)key_of(x) << 32) | (0xffffffffu - (unsigned int)(begin + i));
+        }
+      }
+      __syncthreads();
+      if (listed && me != 0) {                                                    // the first block's list takes them all
+        const int k = sh.list_n;
+        if (tid == 0 && k) sh.ired[0] = atomicAdd(&head->list_n, k);
+        __syncthreads();
+        const int at = sh.ired[0];
+        for (int i = tid; i < k && at + i < SF_CAP; i += SF_THREADS) head->list[at + i] = sh.list[i];
+      }
+      // the first block fills its own list through the same counter, from its own shared memory: no copy
+      if (!whole) {
+        if (mass) publish_sum(s);
+        if (!listed) {
+          // the border bin and those behind it apart: whichever holds the border, fewer tokens remain
+          const double one = warp_sum_d(s_one);
+          const float h1 = warp_max(hi1), l1 = warp_min(lo1), h2 = warp_max(hi2), l2 = warp_min(lo2);
+          if (lane == 0) { sh.red2[warp] = one; sh.fred[0][warp] = h1; sh.fred[1][warp] = l1; sh.fred[2][warp] = h2; sh.fred[3][warp] = l2; }
+          __syncthreads();
+          if (tid < nb) {
+            double o = 0.0;
+            float p1 = -INFINITY, q1 = INFINITY, p2 = -INFINITY, q2 = INFINITY;
+            for (int w = 0; w < SF_WARPS; ++w) {
+              o += sh.red2[w];
+              p1 = fmaxf(p1, sh.fred[0][w]); q1 = fminf(q1, sh.fred[1][w]);
+              p2 = fmaxf(p2, sh.fred[2][w]); q2 = fminf(q2, sh.fred[3][w]);
+            }
+            SampleShared* t = cl.map_shared_rank(&sh, tid);
+            t->pub_sum2[buf][me] = o;
+            t->pub_hi[buf][me] = p1; t->pub_lo[buf][me] = q1; t->pub_hi2[buf][me] = p2; t->pub_lo2[buf][me] = q2;
+          }
+        }
+      }
+      cl.sync();
+      if (whole) {
+        // ---- everything that can be kept is in the first block's list
+        if (me != 0) return;
+        const int cnt = min(sh.list_n, SF_CAP), n2 = pow2_above(cnt);
+        for (int i = cnt + tid; i < n2; i += SF_THREADS) sh.list[i] = 0ull;
+        __syncthreads();
+        sort_falling(sh.list, n2);
+        const int k = K > 0 ? min(K, cnt) : cnt;
+        double w[4], mine = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * tid + j;
+          w[j] = i < k ? w_of(float_of((unsigned int)(sh.list[i] >> 32))) : 0.0;
+          mine += w[j];
+        }
+        double sum;
+        double run = block_scan(mine, sh.red, &sum);
+        const double all = K > 0 ? sum : total;
+        int kept = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * tid + j;
+          if (i < k && w[j] > 0.0 && (!by_mass || run <= top_p * all) && w[j] >= min_p) ++kept;
+          run += w[j];
+        }
+        int m;
+        block_scan_i(kept, sh.ired, &m);
+        if (m == 0) m = 1;
+        // the kept ones by index
+        const int m2 = pow2_above(m);
+        __syncthreads();
+        unsigned long long e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = tid + j * SF_THREADS;
+          e[j] = i < m ? sh.list[i] : 0ull;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = tid + j * SF_THREADS;
+          if (i < m2) sh.list[i] = i < m ? (e[j] << 32) | (e[j] >> 32) : 0ull;    // high half: ~index, falling = index rising
+        }
+        __syncthreads();
+        sort_falling(sh.list, m2);
+        mine = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * tid + j;
+          w[j] = i < m ? w_of(float_of((unsigned int)sh.list[i])) : 0.0;
+          mine += w[j];
+        }
+        run = block_scan(mine, sh.red, &sum);
+        const double goal = fmax((double)a.u[row], 0.0) * sum;
+        int hit = 0x7fffffff;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          run += w[j];
+          if (4 * tid + j < m && run > goal) hit = min(hit, 4 * tid + j);
+        }
+        hit = __reduce_min_sync(0xffffffffu, hit);
+        __syncthreads();
+        if (lane == 0) sh.ired[warp] = hit;
+        __syncthreads();
+        if (tid == 0) {
+          for (int w2 = 1; w2 < SF_WARPS; ++w2) hit = min(hit, sh.ired[w2]);
+          if (hit >= m) hit = m - 1;
+          const unsigned long long v = sh.list[hit];
+          a.out_tok[row] = (int)(0xffffffffu - (unsigned int)(v >> 32));
+          a.out_logp[row] = (float)log(w_of(float_of((unsigned int)v)) / sum);
+        }
+        return;
+      }
+      if (mass) s_above += all_sum();
+      c_above += before;
+      if (listed) {
+        // ---- the undecided ones are in the first block's list: it finds the last value that is kept, and how many have it
+        if (me == 0) {
+          const int cnt = min(sh.list_n, SF_CAP), n2 = pow2_above(cnt);
+          const int extra = limited && thr >= r.lo && thr <= r.hi && bin_of(r, thr) >= b1 && bin_of(r, thr) <= b2 ? ties : 0;
+          for (int i = cnt + tid; i < n2; i += SF_THREADS) sh.list[i] = 0ull;
+          __syncthreads();
+          sort_falling(sh.list, n2);
+          double w[4], mine = 0.0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * tid + j;
+            w[j] = mass && i < cnt ? w_of(float_of((unsigned int)(sh.list[i] >> 32))) : 0.0;
+            mine += w[j];
+          }
+          double sum;
+          double run = s_above + block_scan(mine, sh.red, &sum);
+          int kept = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * tid + j;
+            if (i < cnt && (counting ? c_above + i < K : run <= top_p * total)) ++kept;
+            run += w[j];
+          }
+          int m;
+          block_scan_i(kept, sh.ired, &m);
+          __syncthreads();
+          // all of the list kept, and tokens equal to the top-k's last value behind it: some of those
+          const bool into = m == cnt && extra > 0;
+          const unsigned int last = m > 0 ? (unsigned int)(sh.list[m - 1] >> 32) : 0u;
+          int same = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * tid + j;
+            if (i < m && (unsigned int)(sh.list[i] >> 32) == last) ++same;
+          }
+          int eq;
+          block_scan_i(same, sh.ired, &eq);
+          if (tid < nb) {
+            float t = m > 0 ? float_of(last) : r.hi;
+            if (into) {
+              const double w1 = w_of(thr), have = s_above + sum;
+              const double q = floor((top_p * total - have) / w1) + 1.0;
+              eq = q < 1.0 ? 0 : q > (double)ties ? ties : (int)q;
+              t = thr;
+            }
+            SampleShared* o = cl.map_shared_rank(&sh, tid);
+            o->thr = t;
+            o->ties = eq;
+          }
+        }
+        cl.sync();
+        thr = sh.thr;
+        ties = sh.ties;
+        break;
+      }
+      // ---- too many: the bin of the border, or what is behind it
+      float p1 = -INFINITY, q1 = INFINITY, p2 = -INFINITY, q2 = INFINITY;
+      double one = 0.0;
+      for (int i = 0; i < nb; ++i) {
+        one += sh.pub_sum2[buf][i];
+        p1 = fmaxf(p1, sh.pub_hi[buf][i]); q1 = fminf(q1, sh.pub_lo[buf][i]);
+        p2 = fmaxf(p2, sh.pub_hi2[buf][i]); q2 = fminf(q2, sh.pub_lo2[buf][i]);
+      }
+      if (limited && thr >= r.lo && thr <= r.hi) {                                // the top-k's last value is not in the sums above
+        const int b = bin_of(r, thr);
+        if (b == b1) { one += ties * w_of(thr); p1 = fmaxf(p1, thr); q1 = fminf(q1, thr); }
+        else if (b > b1 && b <= b2) { p2 = fmaxf(p2, thr); q2 = fminf(q2, thr); }
+      }
+      buf ^= 1;
+      if (counting || s_above + one > top_p * total || !(p2 >= q2)) {
+        r = Range{p1, q1, 0.0, false};
+      } else {
+        // what is in the border bin is kept after all; how many those are is only needed for a top-k, which is not cut here
+        s_above += one;
+        r = Range{p2, q2, 0.0, false};
+      }
+      if (round >= 400) {                                                         // not reached by finite arguments: ends the loop whatever they are
+        thr = r.hi;
+        ties = a.V;
+        break;
+      }
+      if (r.hi == r.lo) {                                                         // equal logits all through
+        double q;
+        if (counting) q = (double)(K - c_above);
+        else q = fmin(floor((top_p * total - s_above) / w_of(r.hi)) + 1.0, limited && r.hi == thr ? (double)ties : 1e9);
+        thr = r.hi;
+        ties = (int)fmax(q, 0.0);
+        break;
+      }
+      r.scale = fmax((double)(SF_BINS - 1) / ((double)r.hi - (double)r.lo), it * (double)SF_PER_NAT);
+      for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
+      if (tid == 0) sh.list_n = 0;
+      __syncthreads();
+    }
+    // the histogram and the list are free again: every block has passed a barrier since it last read them
+    cl.sync();
+    for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
+    if (tid == 0) sh.list_n = 0;
+    __syncthreads();
+  }
+
+  // ---- kept weights summed by index: pieces of the block's share, blocks, row
+  const int len = (a.share + SF_SEGS * 32 - 1) / (SF_SEGS * 32) * 32;             // logits of a piece
+  for (int q = 0; q < SF_SEGS / SF_WARPS; ++q) {
+    const int sg = warp * (SF_SEGS / SF_WARPS) + q;
+    double s = 0.0;
+    int eq = 0;
+    for (int i = sg * len + lane; i < min(n, (sg + 1) * len); i += 32) {
+      const float x = xs[i];
+      if (x > thr) {
+        const double w = w_of(x);
+        if (w >= min_p) s += w;
+      } else if (x == thr && x != -INFINITY) {
+        ++eq;
+      }
+    }
+    s = warp_sum_d(s);
+    eq = warp_sum_i(eq);
+    if (lane == 0) { sh.seg_sum[sg] = s; sh.seg_tie[sg] = eq; }
+  }
+  __syncthreads();
+  double w_tie = thr == -INFINITY ? 0.0 : w_of(thr);
+  if (w_tie < min_p) w_tie = 0.0;
+  if (warp == 0) {
+    double s = 0.0;
+    int eq = 0;
+#pragma unroll
+    for (int j = 0; j < SF_SEGS / 32; ++j) { s += sh.seg_sum[lane * (SF_SEGS / 32) + j]; eq += sh.seg_tie[lane * (SF_SEGS / 32) + j]; }
+    s = warp_sum_d(s);
+    eq = warp_sum_i(eq);
+    if (lane < nb) {
+      SampleShared* t = cl.map_shared_rank(&sh, lane);
+      t->pub_sum[buf][me] = s;
+      t->pub_int[buf][me] = eq;
+    }
+  }
+  cl.sync();
+  double sum = 0.0, my_begin = 0.0, my_sum = 0.0;
+  int ties_left = ties, my_ties = 0, last = 0;
+  for (int i = 0; i < nb; ++i) {
+    const int t = min(sh.pub_int[buf][i], ties_left);
+    const double s = sh.pub_sum[buf][i] + t * w_tie;
+    if (i == me) { my_begin = sum; my_sum = s; my_ties = ties_left; }
+    if (s > 0.0) last = i;
+    sum += s;
+    ties_left -= t;
+  }
+  const double goal = fmax((double)a.u[row], 0.0) * sum;
+  // the first block whose end passes the goal (the last one with any weight, should rounding leave none)
+  const bool mine = my_sum > 0.0 && my_begin <= goal && (my_begin + my_sum > goal || me == last);
+  if (!mine || warp != 0) return;
+  double run = my_begin;
+  int left = my_ties, sg = -1, sg_left = 0;
+  double sg_run = 0.0;
+  for (int i = 0; i < SF_SEGS; ++i) {                                             // every lane the same
+    const int t = min(sh.seg_tie[i], left);
+    const double s = sh.seg_sum[i] + t * w_tie;
+    if (s > 0.0) { sg = i; sg_run = run; sg_left = left; }
+    run += s;
+    left -= t;
+    if (s > 0.0 && run > goal) break;
+  }
+  int tok = -1;
+  double w_tok = 0.0;
+  run = sg_run;
+  left = sg_left;
+  for (int i0 = sg * len; i0 < min(n, (sg + 1) * len); i0 += 32) {
+    const int i = i0 + lane;
+    const float x = i < min(n, (sg + 1) * len) ? xs[i] : -INFINITY;
+    const unsigned int eq = __ballot_sync(0xffffffffu, x == thr && x != -INFINITY);
+    const int rank = __popc(eq & ((1u << lane) - 1u));
+    double w = 0.0;
+    if (x > thr) { w = w_of(x); if (w < min_p) w = 0.0; }
+    else if ((eq >> lane & 1u) && rank < left) w = w_tie;
+    double s = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += t;
+    }
+    const unsigned int some = __ballot_sync(0xffffffffu, w > 0.0), hit = __ballot_sync(0xffffffffu, w > 0.0 && run + s > goal);
+    if (some) {
+      const int from = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+      tok = begin + i0 + from;
+      w_tok = __shfl_sync(0xffffffffu, w, from);
+    }
+    if (hit) break;
+    run += __shfl_sync(0xffffffffu, s, 31);
+    left -= min(left, __popc(eq));
+  }
+  if (lane == 0) {
+    a.out_tok[row] = tok;
+    a.out_logp[row] = (float)log(w_tok / sum);
+  }
+}
+
+}  // namespace ab2
+
+extern "C" {
+using namespace ab2;
+
+// logits [B, V] fp32, rows `ld` elements apart; u, inv_temp (> 0), top_p, min_p fp32 [B]; top_k, greedy int32 [B] (greedy may be null).
+// top_k <= 0, top_p >= 1, min_p <= 0 switch a filter off. A row in which nothing has weight gives token -1 and log-prob -inf.
+int ab2_sample_filtered(const void* logits, long long ld, int B, int V, const void* u, const void* inv_temp, const int* top_k, const void* top_p,
+                        const void* min_p, const int* greedy, int* out_tok, float* out_logp, void* stream) {
+  if (B <= 0) return 0;
+  if (V <= 0 || ld < V) return 10;
+  int nb = 1;
+  while (nb < SF_MAX_CLUSTER && (V + nb - 1) / nb > 20480) nb *= 2;              // two blocks an SM as long as a share is below 80 KB
+  SampleArgs a;
+  a.share = ((V + nb - 1) / nb + 3) / 4 * 4;
+  const int head = (int)((sizeof(SampleShared) + 15) / 16 * 16), smem = head + a.share * 4;
+  if (smem > 227 * 1024) return 11;
+  if ((long long)B * nb > 0x7fffffffLL) return 10;
+  a.logits = (const float*)logits; a.ld = ld; a.u = (const float*)u; a.inv_temp = (const float*)inv_temp; a.top_p = (const float*)top_p;
+  a.min_p = (const float*)min_p; a.top_k = top_k; a.greedy = greedy; a.out_tok = out_tok; a.out_logp = out_logp; a.V = V;
+  a.aligned = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
+  static ab2host::DevState st;
+  if (ab2host::prepare_launch(sample_filtered_kernel, 227 * 1024, st, nullptr)) return 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(B * nb);
+  cfg.blockDim = dim3(SF_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = nb; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (ab2host::pdl_enabled()) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, sample_filtered_kernel, a) == cudaSuccess ? 0 : 1;
+}
+}
