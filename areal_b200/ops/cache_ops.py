@@ -54,33 +54,47 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _check_pages(p: QuantPages, dim: int, dev) -> None:
-    s = p.k.shape
-    _need(p.k.dtype == F8 and p.v.dtype == F8 and len(s) == 4 and p.v.shape == s, "codes: two e4m3 tensors [pages, Hkv, page_size, D]")
-    _need(p.k.is_contiguous() and p.v.is_contiguous(), "codes have to be contiguous")
-    _need(p.k_scale.dtype == torch.float32 and p.v_scale.dtype == torch.float32 and p.k_scale.shape == s[:2] and p.v_scale.shape == s[:2]
-          and p.k_scale.is_contiguous() and p.v_scale.is_contiguous(), "scales: two contiguous fp32 tensors [pages, Hkv]")
+def _check_pages(p: QuantPages, dim: int, dev: int) -> tuple:
+    """(pages, Hkv, page size) of a cache on device number ``dev`` (-1: the host), after its checks."""
+    k, v, ks, vs = p.k, p.v, p.k_scale, p.v_scale
+    s = k.shape
+    if (len(s) == 4 and v.shape == s and k.dtype is F8 and v.dtype is F8 and ks.dtype is torch.float32 and vs.dtype is torch.float32 and ks.shape == s[:2]
+            and vs.shape == s[:2] and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and s[2] in PAGE_SIZES
+            and s[3] == dim and (dim == 128 or dim == 64) and s[0] > 0 and s[1] > 0
+            and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == dev):
+        return s[0], s[1], s[2]
+    # which of them it is
+    _need(k.dtype == F8 and v.dtype == F8 and len(s) == 4 and v.shape == s, "codes: two e4m3 tensors [pages, Hkv, page_size, D]")
+    _need(k.is_contiguous() and v.is_contiguous(), "codes have to be contiguous")
+    _need(ks.dtype == torch.float32 and vs.dtype == torch.float32 and ks.shape == s[:2] and vs.shape == s[:2] and ks.is_contiguous() and vs.is_contiguous(),
+          "scales: two contiguous fp32 tensors [pages, Hkv]")
     _need(s[3] == dim and dim in (64, 128), f"head size {dim} with a cache of {s[3]}: 64 or 128 are built")
     _need(s[2] in PAGE_SIZES, f"page size {s[2]}: one of {PAGE_SIZES}")
     _need(s[0] > 0 and s[1] > 0, "a cache without pages or heads")
-    _need(p.k.device == dev and p.v.device == dev and p.k_scale.device == dev and p.v_scale.device == dev, "cache on another device than the rows")
+    raise ValueError("cache on another device than the rows")
 
 
-def _check_table(table, lens, dev) -> None:
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.shape[1] > 0, "page table: contiguous int32 [B, width]")
-    _need(lens.dtype == torch.int32 and lens.is_contiguous() and lens.shape == table.shape[:1], "lengths: contiguous int32 [B]")
-    _need(table.device == dev and lens.device == dev, "page table or lengths on another device")
+def _check_table(table, lens, B: int, dev: int) -> int:
+    """The table's width, after its checks."""
+    t = table.shape
+    if (len(t) == 2 and t[0] == B and t[1] > 0 and table.dtype is torch.int32 and lens.dtype is torch.int32 and lens.shape == t[:1] and table.is_contiguous()
+            and lens.is_contiguous() and table.get_device() == lens.get_device() == dev):
+        return t[1]
+    _need(len(t) == 2 and table.dtype == torch.int32 and table.is_contiguous() and t[1] > 0, "page table: contiguous int32 [B, width]")
+    _need(t[0] == B, f"a table of {t[0]} sequences for {B}")
+    _need(lens.dtype == torch.int32 and lens.is_contiguous() and lens.shape == t[:1], "lengths: contiguous int32 [B]")
+    raise ValueError("page table or lengths on another device")
 
 
-def _launch(t: torch.Tensor, name: str, *args) -> None:
-    """Calls a launcher on the device of ``t`` and its current stream."""
-    dev = t.device
-    if dev.index == torch.cuda.current_device():
-        rc = getattr(_lib.get_lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+def _launch(dev: int, name: str, *args) -> None:
+    """Calls a launcher on device number ``dev`` and its current stream."""
+    if dev == torch._C._cuda_getDevice():
+        rc = getattr(_lib.get_lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = getattr(_lib.get_lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, name)
+            rc = getattr(_lib.get_lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 # ----------------------------------------------------------------------------- append
@@ -135,31 +149,35 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pages: QuantPages, page_table: 
     may be a part of a wider projection (``k.stride(0)`` a multiple of 8 elements, heads dense). A page that gets rows belongs to one
     sequence. ``page_table`` ``[B, width]`` int32; entries of a sequence beyond its length are not read. An entry out of the cache, or a
     length beyond the table, sets the device error word (code 6) and writes nothing for that page."""
-    _need(k.dim() == 3 and k.shape == v.shape and k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16, "keys and values: bf16 [rows, Hkv, D]")
-    dev, (rows, Hkv, D) = k.device, k.shape
-    _need(v.device == dev, "keys and values on different devices")
-    _check_pages(pages, D, dev)
-    _check_table(page_table, seq_lens, dev)
-    B = page_table.shape[0]
-    _need(pages.k.shape[1] == Hkv, f"rows of {Hkv} heads into a cache of {pages.k.shape[1]}")
+    shape = k.shape
+    if not (len(shape) == 3 and v.shape == shape and k.dtype is torch.bfloat16 and v.dtype is torch.bfloat16):
+        raise ValueError("keys and values: bf16 [rows, Hkv, D]")
+    dev, (rows, Hkv, D) = k.get_device(), shape
+    if v.get_device() != dev:
+        raise ValueError("keys and values on different devices")
+    P, heads, ps = _check_pages(pages, D, dev)
+    if heads != Hkv:
+        raise ValueError(f"rows of {Hkv} heads into a cache of {heads}")
     if cu_seqlens is None:
-        _need(rows == B, f"{rows} rows for {B} sequences")
+        B, cu = rows, None
     else:
-        _need(cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.shape == (B + 1,) and cu_seqlens.device == dev,
+        B, cu = cu_seqlens.numel() - 1, cu_seqlens.data_ptr()
+        _need(B >= 0 and cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous() and cu_seqlens.get_device() == dev,
               "cu_seqlens: contiguous int32 [B + 1]")
-    if not k.is_cuda:
+    width = _check_table(page_table, seq_lens, B, dev)
+    if dev < 0:
         return kv8_append_ref(k, v, pages, page_table, seq_lens, cu_seqlens)
     if rows == 0 or B == 0:
         return
     ks, vs = k.stride(), v.stride()
-    _need(ks[2] == 1 and vs[2] == 1 and (Hkv == 1 or (ks[1] == D and vs[1] == D)), "heads of a row have to be dense")
-    if rows == 1:
-        ks = vs = (Hkv * D,)
+    kr, vr = (ks[0], vs[0]) if rows > 1 else (0, 0)
     kp, vp = k.data_ptr(), v.data_ptr()
-    _need(ks[0] % 8 == 0 and vs[0] % 8 == 0 and (kp | vp) % 16 == 0, "rows have to start on 16 bytes")
-    _launch(k, "ab2_kv8_append", kp, vp, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), page_table.data_ptr(),
-            seq_lens.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), B, rows, Hkv, D, pages.k.shape[2], page_table.shape[1],
-            pages.k.shape[0], ks[0], vs[0])
+    if not (ks[2] == 1 and vs[2] == 1 and (Hkv == 1 or (ks[1] == D and vs[1] == D))):
+        raise ValueError("heads of a row have to be dense")
+    if (kr | vr) & 7 or (kp | vp) & 15:
+        raise ValueError("rows have to start on 16 bytes")
+    _launch(dev, "ab2_kv8_append", kp, vp, pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), page_table.data_ptr(),
+            seq_lens.data_ptr(), cu, B, rows, Hkv, D, ps, width, P, kr, vr)
 
 
 # ----------------------------------------------------------------------------- attention of single tokens
@@ -181,9 +199,25 @@ def kv8_decode_ref(q, pages: QuantPages, page_table, seq_lens, scale: Optional[f
 
 
 @functools.lru_cache(maxsize=256)
-def _decode_workspace(dev: int, *sizes: int) -> int:
+def _decode_workspace(dev: int, *sizes: int) -> tuple[int, int]:
+    """(bytes of the workspace, number of counters) for these sizes."""
+    n = ctypes.c_int(0)
     with torch.cuda.device(dev):
-        return int(_lib.get_lib().ab2_kv8_decode_workspace(*sizes))
+        return int(_lib.get_lib().ab2_kv8_decode_workspace(*sizes, ctypes.addressof(n))), n.value
+
+
+_COUNTERS: dict = {}        # (device, stream) -> zeros that every call on the stream leaves zero
+
+
+def _counters(dev: int, n: int) -> torch.Tensor:
+    """Zeros that calls on the current stream may share, one after the other; a captured call gets its own, cleared in its graph."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(n, dtype=torch.int32, device=f"cuda:{dev}")
+    key = dev, torch._C._cuda_getCurrentRawStream(dev)
+    c = _COUNTERS.get(key)
+    if c is None or c.numel() < n:
+        c = _COUNTERS[key] = torch.zeros(max(n, 1024), dtype=torch.int32, device=f"cuda:{dev}")
+    return c
 
 
 def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq_lens: torch.Tensor, scale: Optional[float] = None,
@@ -194,32 +228,39 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous, where given);
     a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
     length beyond the table, sets the device error word (code 6); the row's result is not to be used. The workspace is allocated in
-    the call, on the current stream, so calls on several streams and captured graphs do not share one. At most 8192 sequences."""
-    _need(q.dim() == 3 and q.dtype == torch.bfloat16, "queries: bf16 [B, Hq, D]")
-    dev, (B, Hq, D) = q.device, q.shape
-    _check_pages(pages, D, dev)
-    _check_table(page_table, seq_lens, dev)
-    P, Hkv, ps, _ = pages.k.shape
-    width = page_table.shape[1]
-    _need(page_table.shape[0] == B, f"{B} queries for {page_table.shape[0]} sequences")
-    _need(Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads over {Hkv} cached ones")
-    _need(B <= 8192 and width * ps < (1 << 31) - 64, "more than 8192 sequences, or a table wider than 2^31 tokens")
+    the call, and the counters belong to the stream or, in a captured call, to its graph: calls on several streams and graphs share neither. At most
+    8192 sequences."""
+    shape = q.shape
+    if not (len(shape) == 3 and q.dtype is torch.bfloat16):
+        raise ValueError("queries: bf16 [B, Hq, D]")
+    dev, (B, Hq, D) = q.get_device(), shape
+    P, Hkv, ps = _check_pages(pages, D, dev)
+    width = _check_table(page_table, seq_lens, B, dev)
+    if Hq <= 0 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads over {Hkv} cached ones")
+    if B > 8192 or width * ps >= (1 << 31) - 64:
+        raise ValueError("more than 8192 sequences, or a table wider than 2^31 tokens")
     if out is not None:
-        _need(out.shape == q.shape and out.dtype == torch.bfloat16 and out.is_contiguous() and out.device == dev, "out: contiguous bf16 like the queries")
-    if not q.is_cuda:
+        _need(out.shape == shape and out.dtype == torch.bfloat16 and out.is_contiguous() and out.get_device() == dev, "out: contiguous bf16 like the queries")
+    if scale is None:
+        scale = D ** -0.5
+    if dev < 0:
         o = kv8_decode_ref(q, pages, page_table, seq_lens, scale).to(torch.bfloat16)
         return o if out is None else out.copy_(o)
     if out is None:
-        out = torch.empty(B, Hq, D, dtype=torch.bfloat16, device=dev)
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
     if B == 0:
         return out
     st = q.stride()
-    _need(st[2] == 1 and (Hq == 1 or st[1] == D), "heads of a row have to be dense")
-    row = st[0] if B > 1 else Hq * D
-    _need(row % 8 == 0 and q.data_ptr() % 16 == 0, "rows have to start on 16 bytes")
-    ws = torch.empty(_decode_workspace(dev.index, B, Hq, Hkv, D, ps, width), dtype=torch.uint8, device=dev)
-    _launch(q, "ab2_kv8_decode", q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
-            page_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, ps, width, P, D ** -0.5 if scale is None else scale, row)
+    row = st[0] if B > 1 else 0
+    if not (st[2] == 1 and (Hq == 1 or st[1] == D)):
+        raise ValueError("heads of a row have to be dense")
+    if row & 7 or q.data_ptr() & 15:
+        raise ValueError("rows have to start on 16 bytes")
+    size, n = _decode_workspace(dev, B, Hq, Hkv, D, ps, width)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _launch(dev, "ab2_kv8_decode", q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
+            page_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), _counters(dev, n).data_ptr(), B, Hq, Hkv, D, ps, width, P, scale, row)
     return out
 
 
@@ -283,10 +324,10 @@ def copy_pages(buffers: Sequence[tuple], src, dst, tokens=None) -> None:
     pairs = np.empty((n, 3), np.int32)
     pairs[:, 0], pairs[:, 1], pairs[:, 2] = src, dst, -1 if tokens is None else tokens
     flat = (ctypes.c_longlong * len(desc))(*desc)
-    _launch(buffers[0][0], "ab2_copy_pages", ctypes.addressof(flat), len(buffers), pairs.ctypes.data, n)
+    _launch(dev.index, "ab2_copy_pages", ctypes.addressof(flat), len(buffers), pairs.ctypes.data, n)
 
 
 _lib.declare("ab2_kv8_append", [_V] * 9 + [_I] * 7 + [_L, _L, _V])
-_lib.declare("ab2_kv8_decode", [_V] * 9 + [_I] * 7 + [_F, _L, _V])
-_lib.declare("ab2_kv8_decode_workspace", [_I] * 6, _L)
+_lib.declare("ab2_kv8_decode", [_V] * 10 + [_I] * 7 + [_F, _L, _V])
+_lib.declare("ab2_kv8_decode_workspace", [_I] * 6 + [_V], _L)
 _lib.declare("ab2_copy_pages", [_V, _I, _V, _I, _V])

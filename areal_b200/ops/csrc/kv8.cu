@@ -191,17 +191,21 @@ kv8_append_page_kernel(Kv8Args a, const int* __restrict__ table, const int* __re
 // ------------------------------------------------------------------ attention of single tokens
 // o = softmax(scale * q K^T) V over the first lens[b] tokens, G query heads for each key/value head. Bound by the codes' bytes.
 //
-// Split: the tokens of all (sequence, head) items are cut into chunks of 64 and the chunks, in order, dealt evenly to the blocks of
-// one resident wave, whatever the lengths are; a block that ends inside an item leaves (m, l, o) for the join kernel.
-// Warp w of a block takes tokens 16 w .. 16 w + 15 of each chunk. Its codes go from global memory straight into the registers
-// that the matrix instruction wants, one tile ahead, so there is no shared-memory round trip and no barrier in the loop:
-//   S^T[16 tokens, 8 heads] = K Q^T: the sum over dims may be taken in any order, so a thread's 16 contiguous bytes of a row serve as
+// Split: every (sequence, head) item is cut into units of U chunks of 64 tokens, U from the whole batch's tokens so that a resident wave of
+// blocks gets about KV8_ROUNDS units each, whatever the lengths are. Blocks take units from a counter: SMs do not get equal shares of the
+// memory's rate (the slowest of equal static shares ended 20 % after the mean), so the faster ones take more. The block that
+// finishes the last unit of an item joins its parts. Both kinds of counters wrap to zero with the last count, so they are left as found.
+// Warp w of a block takes tokens 16 w .. 16 w + 15 of each chunk and fetches them itself, with 16-byte asynchronous copies into a ring
+// of its own in shared memory, so there is no barrier in the loop and the bytes in flight are not bounded by registers.
+//   S^T[16 tokens, 8 heads] = K Q^T: the sum over dims may be taken in any order, so 16 contiguous bytes of a row serve a thread as
 //     four steps of k = 16 (the queries are laid out to match);
 //   O^T[D dims, 8 heads] += V^T P^T: rows (dims) may stand in any order too, so a thread's 16 contiguous dims of four tokens are
 //     paired by byte permutes; P^T comes from S^T by an 8 x 8 transpose between registers.
-// e4m3 converts to fp16 exactly; q is divided by a power of two for its head (exact), P is rounded to fp16 (11 bits, half a step
-// 2^-12) around a running maximum that is only moved when a score passes it by 2^6, and both sums are fp32.
-constexpr int KV8_CHUNK = 64;
+// The 16-byte pieces of a 128-byte line stand where their number is xor-ed with the line's, so that both patterns of reads are free of
+// bank conflicts. e4m3 converts to fp16 exactly; q is divided by a power of two for its head (exact), P is rounded to fp16 (11 bits,
+// half a step 2^-12) as e^x scaled so that the largest seen lies between 2^9 and 2^15 (the running maximum only moves when a score leaves
+// that range, so that shares down to 2^-23 of the largest keep all bits), and both sums are fp32.
+constexpr int KV8_CHUNK = 64, KV8_ROUNDS = 1, KV8_MOST_ROWS = 8192;
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -227,15 +231,23 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint4 ldg_stream16(const void* p) {
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p));
   return v;
 }
-__device__ __forceinline__ uint2 ldg_stream8(const void* p) {
+__device__ __forceinline__ uint2 lds8(uint32_t p) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p));
   return v;
+}
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 struct Kv8Decode {
@@ -244,84 +256,151 @@ struct Kv8Decode {
   const float *ks, *vs;
   const int *table, *lens;
   __nv_bfloat16* out;
-  float *part_o, *part_ml;      // [2 * grid][HP][D], [2 * grid][HP][2]
-  int* meta;                    // [items]: how the item is split, for the join kernel
+  float *part_o, *part_ml;      // [slots][HP][D], [slots][HP][2]: units of items that are split
+  unsigned int* counters;       // [1 + items], zero: units taken, and units finished of each item
   int* err;
-  int B, Hq, Hkv, G, groups, page_size, width, num_pages;
+  int B, Hq, Hkv, G, groups, page_size, page_bits, width, num_pages;
   float scale_log2;             // softmax scale * log2(e)
   long long q_stride;
 };
 
-// Codes of one 16-token tile in a thread's registers.
+// Where piece `c` (16 bytes) of row `r` stands in a 16-row tile.
 template <int D>
-struct Kv8Tile {
-  uint32_t k[2][D / 16];        // tokens gq and gq + 8: D / 64 pieces of 16 bytes at dims 64 c + 16 tq
-  uint32_t v[4][D / 32];        // tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: D / 8 bytes at dim gq * D / 8
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  if constexpr (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
+  return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ ((r & 6))) << 4);            // two rows in a line; line r / 2, xor 2 * (line % 4)
+}
+
+template <int D, int NT>
+struct Kv8Cfg {
+  static constexpr int BLOCKS = NT == 1 ? 4 : 2;           // resident on an SM
+  static constexpr int STAGES = NT == 1 ? 3 : 4;           // of each warp's ring: 4 KB at D = 128
+  static constexpr int TILE = 16 * D;                      // bytes of one operand
+  static constexpr int RING = (STAGES * 2 * TILE > 8 * NT * (D + 4) * 4 ? STAGES * 2 * TILE : (8 * NT * (D + 4) * 4 + 127) / 128 * 128);
 };
 
 template <int D, int NT>        // NT: tiles of 8 query heads
-__global__ void __launch_bounds__(128, NT == 1 ? 3 : 2)
-kv8_decode_kernel(Kv8Decode a) {
+__global__ void __launch_bounds__(128, Kv8Cfg<D, NT>::BLOCKS)
+kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
+  using Cfg = Kv8Cfg<D, NT>;
   constexpr int HP = 8 * NT;
   constexpr int KS = D / 16;            // steps of S; also D / 16 row tiles of O
-  extern __shared__ __align__(16) unsigned char dsm[];
-  float* mo = reinterpret_cast<float*>(dsm);                  // [4][HP][D + 4]
-  float* mm = mo + 4 * HP * (D + 4);                          // [4][HP]
+  constexpr int S = Cfg::STAGES;
+  extern __shared__ __align__(128) unsigned char dsm[];       // four rings; where a segment ends, each holds its warp's result [HP][D + 4]
+  float* mm = reinterpret_cast<float*>(dsm + 4 * Cfg::RING);  // [4][HP]
   float* ml = mm + 4 * HP;                                    // [4][HP]
-  int* prefix = reinterpret_cast<int*>(ml + 4 * HP);          // [B + 1] chunks before sequence b
-  __shared__ int wsum[4];
+  int* units = reinterpret_cast<int*>(ml + 4 * HP);           // [B + 1] units of one head before sequence b
+  int* slots = units + a.B + 1;                               // [B + 1] those of split items only
+  __shared__ int wsum[2][4], s_next, s_last;
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
   const int Hv = a.Hkv * a.groups;
+  const uint32_t ring = smem_u32(dsm) + warp * Cfg::RING;
+  const uint32_t in_off = tile_at<D>(lane / (D / 16), lane % (D / 16)), k_off = tile_at<D>(gq, (D / 64) * tq);
+  const uint32_t v_off = D == 128 ? tile_at<D>(2 * tq, gq) : tile_at<D>(2 * tq, gq >> 1) + 8 * (gq & 1);
   const int room = a.width * a.page_size;
   auto length = [&](int b) { return min(max(a.lens[b], 0), room); };
-  // ---- chunks of the sequences before each, the whole batch in every block (a few loads a thread)
+  // ---- chunks of the batch, and with them the size of a unit: every block counts them all (a few loads a thread)
+  int sum = 0;
+  for (int i = tid; i < a.B; i += 128) {
+    if (blockIdx.x == 0 && a.lens[i] > room) set_error(a.err, ERR_BOUNDS);
+    const int n = (length(i) + KV8_CHUNK - 1) / KV8_CHUNK;
+    units[i] = n;
+    sum += n;
+  }
+  sum = __reduce_add_sync(0xffffffffu, sum);
+  if (lane == 0) wsum[0][warp] = sum;
+  __syncthreads();
+  const int chunks = (wsum[0][0] + wsum[0][1] + wsum[0][2] + wsum[0][3]) * Hv;
+  const int U = max(1, (int)(((unsigned)chunks + gridDim.x * KV8_ROUNDS - 1) / (gridDim.x * KV8_ROUNDS)));
   {
-    int carry = 0;
+    int carry_u = 0, carry_s = 0;
     for (int i0 = 0; i0 < a.B; i0 += 128) {
       const int i = i0 + tid;
-      if (i < a.B && blockIdx.x == 0 && a.lens[i] > room) set_error(a.err, ERR_BOUNDS);
-      const int n = i < a.B ? (length(i) + KV8_CHUNK - 1) / KV8_CHUNK : 0;
-      int s = n;
+      const int np = i < a.B ? (units[i] + U - 1) / U : 0, sp = np > 1 ? np : 0;
+      int u = np, s = sp;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
+        const int x = __shfl_up_sync(0xffffffffu, u, o), y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) { u += x; s += y; }
       }
-      if (lane == 31) wsum[warp] = s;
       __syncthreads();
-      int before = carry;
-      for (int w = 0; w < warp; ++w) before += wsum[w];
-      if (i < a.B) prefix[i] = before + s - n;
-      carry += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+      if (lane == 31) { wsum[0][warp] = u; wsum[1][warp] = s; }
       __syncthreads();
+      int bu = carry_u, bs = carry_s;
+      for (int w = 0; w < 4; ++w) {
+        if (w < warp) { bu += wsum[0][w]; bs += wsum[1][w]; }
+        carry_u += wsum[0][w]; carry_s += wsum[1][w];
+      }
+      if (i < a.B) { units[i] = bu + u - np; slots[i] = bs + s - sp; }
     }
-    if (tid == 0) prefix[a.B] = carry;
+    if (tid == 0) { units[a.B] = carry_u; slots[a.B] = carry_s; }
     __syncthreads();
   }
-  const long long total = (long long)prefix[a.B] * Hv;
-  const long long grid = min((long long)gridDim.x, total);      // blocks with a share: none of them is empty
-  if (blockIdx.x >= grid) return;
-  long long pos = total * blockIdx.x / grid;
-  const long long stop = total * (blockIdx.x + 1) / grid;
-  bool first_segment = true;
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)            // rows without tokens
+    if (units[b] == units[b + 1])
+      for (int i = tid; i < a.Hq * D / 8; i += 128) reinterpret_cast<uint4*>(a.out + (size_t)b * a.Hq * D)[i] = make_uint4(0u, 0u, 0u, 0u);
+  const int total = units[a.B] * Hv;                            // units
+  const int grid = min((int)gridDim.x, total);
 
-  while (pos < stop) {
+  for (int unit = blockIdx.x; unit < total;) {
+    // the next one: every block asks once more than it gets, so there are `total` counts in all
+    unsigned int next = 0;
+    if (tid == 0) next = grid + atomicInc(a.counters, total - 1);
     // ---- which item, which of its chunks
-    int lo = 0, hi = a.B;                                     // last b with Hv * prefix[b] <= pos and chunks of its own
+    int lo = 0, hi = a.B;                                       // last b with Hv * units[b] <= unit and units of its own
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((long long)prefix[mid] * Hv <= pos) lo = mid; else hi = mid;
+      if (units[mid] * Hv <= unit) lo = mid; else hi = mid;
     }
-    const int b = lo, nc = prefix[b + 1] - prefix[b];
-    const long long base = (long long)prefix[b] * Hv;
-    const int hv = (int)((pos - base) / nc);
-    const long long item0 = base + (long long)hv * nc;
-    const int c0 = (int)(pos - item0), c1 = (int)min((long long)nc, stop - item0);
+    const int b = lo, np = units[b + 1] - units[b], rest = unit - units[b] * Hv, hv = rest / np, part = rest - hv * np;
+    const int len = length(b), nc = (len + KV8_CHUNK - 1) / KV8_CHUNK, per = (nc + np - 1) / np;
+    const int c0 = part * per, c1 = min(nc, c0 + per);
     const int h = hv / a.groups, g0 = (hv - h * a.groups) * 16, ng = min(a.G - g0, HP);
-    const int len = length(b);
     const int* pt = a.table + (size_t)b * a.width;
+
+    // ---- this warp's tiles: tokens 64 c + 16 warp of chunks c0 .. c1
+    const int t_first = c0 * KV8_CHUNK + warp * 16;
+    const int n_tiles = min(c1 - c0, max(0, (len - t_first + KV8_CHUNK - 1) / KV8_CHUNK));
+    // Lane i of a block of 32 tiles holds its page (fetched one block ahead), and later its scales (from when its first tile is fetched).
+    int pg = 0, pg_next = 0;
+    float ksc = 0.f, vsc = 0.f, ksc_next = 0.f, vsc_next = 0.f;
+    auto page_of = [&](int i) {
+      int p = 0;
+      if (i < n_tiles) {
+        p = pt[(t_first + i * KV8_CHUNK) >> a.page_bits];
+        if ((unsigned)p >= (unsigned)a.num_pages) { set_error(a.err, ERR_BOUNDS); p = 0; }
+      }
+      return p;
+    };
+    uint32_t st_in = ring, st_out = ring;                       // stages that the next tile goes to and comes from
+    auto fetch = [&](int i) {                                   // tile i into its stage; an empty group where there is none
+      if (i < n_tiles) {
+        if ((i & 31) == 0) {
+          pg = pg_next;
+          ksc_next = a.ks[(size_t)pg * a.Hkv + h];
+          vsc_next = a.vs[(size_t)pg * a.Hkv + h];
+          pg_next = page_of(i + 32 + lane);
+        }
+        const int p = __shfl_sync(0xffffffffu, pg, i & 31);
+        const int t = (t_first + i * KV8_CHUNK) & (a.page_size - 1);
+        const size_t at = ((((size_t)p * a.Hkv + h) << a.page_bits) + t) * D + lane * 16;
+        const unsigned char *ksrc = a.kc + at, *vsrc = a.vc + at;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {                      // 512 bytes of each, contiguous
+          // D = 128: 4 rows on, which flips bit 2 of a line's xor; D = 64: 8 rows, 4 lines on, which leaves it
+          const uint32_t d = st_in + (D == 128 ? in_off ^ ((j & 1) << 6) : in_off) + j * 512;
+          copy16_async(d, ksrc + j * 512);
+          copy16_async(d + Cfg::TILE, vsrc + j * 512);
+        }
+        st_in = st_in == ring + (S - 1) * 2 * Cfg::TILE ? ring : st_in + 2 * Cfg::TILE;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    pg_next = page_of(lane);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) fetch(i);
 
     // ---- queries as the B operand: head gq of the tile, dims in the order of the keys' bytes
     uint32_t qf[NT][KS][2];
@@ -334,7 +413,7 @@ kv8_decode_kernel(Kv8Decode a) {
       const __nv_bfloat16* qp = a.q + (size_t)b * a.q_stride + (size_t)(h * a.G + g0 + hd) * D;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const uint2 w = hd < ng ? *reinterpret_cast<const uint2*>(qp + (s >> 2) * 64 + tq * 16 + (s & 3) * 4) : make_uint2(0u, 0u);
+        const uint2 w = hd < ng ? *reinterpret_cast<const uint2*>(qp + (D == 128 ? tq * 32 : tq * 16) + s * 4) : make_uint2(0u, 0u);
         raw[s][0] = w.x; raw[s][1] = w.y;
         const float2 x = unpack_bf16(w.x), y = unpack_bf16(w.y);
         m = fmaxf(m, fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(y.x), finite_abs(y.y))));
@@ -363,144 +442,121 @@ kv8_decode_kernel(Kv8Decode a) {
       l_run[t][0] = l_run[t][1] = 0.f;
     }
 
-    // ---- this warp's tiles: tokens 64 c + 16 warp of chunks c0 .. c1
-    const int t_first = c0 * KV8_CHUNK + warp * 16;
-    const int n_tiles = min(c1 - c0, max(0, (len - t_first + KV8_CHUNK - 1) / KV8_CHUNK));
-    int pg = 0, pg_next = 0;                                   // lane i: page of tile 32 k + i
-    float ksc = 0.f, vsc = 0.f;
-    auto page_of = [&](int i) {
-      int p = 0;
-      if (i < n_tiles) {
-        p = pt[(t_first + i * KV8_CHUNK) / a.page_size];
-        if (p < 0 || p >= a.num_pages) { set_error(a.err, ERR_BOUNDS); p = 0; }
-      }
-      return p;
-    };
-    auto load = [&](int i, Kv8Tile<D>& x) {
-      const int p = __shfl_sync(0xffffffffu, pg, i & 31);
-      const int t = (t_first + i * KV8_CHUNK) % a.page_size;
-      const size_t at = (((size_t)p * a.Hkv + h) * a.page_size + t) * D;
-      const unsigned char* kp = a.kc + at + gq * D + tq * 16;
-      const unsigned char* vp = a.vc + at + 2 * tq * D + gq * (D / 8);
+    float v_last = 0.f;
+    uint32_t ratio = 0u;                                        // scale of this page's values over v_ref, as two fp16
+    auto work = [&](int i) {
+      if ((i & 31) == 0) { ksc = ksc_next; vsc = vsc_next; }
+      const float kscale = __shfl_sync(0xffffffffu, ksc, i & 31), vscale = __shfl_sync(0xffffffffu, vsc, i & 31);
+      const int left = len - (t_first + i * KV8_CHUNK);         // tokens of the tile that exist (16 or more: all)
+      const uint32_t kt = st_out, vt = st_out + Cfg::TILE;
+      st_out = st_out == ring + (S - 1) * 2 * Cfg::TILE ? ring : st_out + 2 * Cfg::TILE;
+      uint32_t k[2][D / 16], v[4][D / 32];
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          *reinterpret_cast<uint4*>(&x.k[r][4 * c]) = ldg_stream16(kp + r * 8 * D + c * 64);
+        for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint4*>(&k[r][4 * c]) = lds16(kt + (k_off ^ (c << 4)) + r * 8 * D);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const unsigned char* p4 = vp + ((r >> 1) * 8 + (r & 1)) * D;
-        if constexpr (D == 128) *reinterpret_cast<uint4*>(&x.v[r][0]) = ldg_stream16(p4);
-        else *reinterpret_cast<uint2*>(&x.v[r][0]) = ldg_stream8(p4);
+        if constexpr (D == 128) *reinterpret_cast<uint4*>(&v[r][0]) = lds16(vt + (v_off ^ ((r & 1) << 4)) + (r & 1) * 128 + (r >> 1) * 1024);
+        else *reinterpret_cast<uint2*>(&v[r][0]) = lds8(vt + (v_off ^ ((r & 1) << 6)) + (r >> 1) * 512);
       }
-    };
-    auto work = [&](int i, Kv8Tile<D>& x) {
-      const float kscale = __shfl_sync(0xffffffffu, ksc, i & 31), vscale = __shfl_sync(0xffffffffu, vsc, i & 31);
-      const int left = len - (t_first + i * KV8_CHUNK);         // tokens of the tile that exist (16 or more: all)
       float s[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        const uint32_t a0 = half2_lo(x.k[0][j]), a2 = half2_hi(x.k[0][j]), a1 = half2_lo(x.k[1][j]), a3 = half2_hi(x.k[1][j]);
+        const uint32_t a0 = half2_lo(k[0][j]), a2 = half2_hi(k[0][j]), a1 = half2_lo(k[1][j]), a3 = half2_hi(k[1][j]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) mma_f16_16816(s[t], a0, a1, a2, a3, qf[t][j][0], qf[t][j][1]);
-      }
-      bool grow = false;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float f0 = qs[t][0] * kscale, f1 = qs[t][1] * kscale;
-        s[t][0] = gq < left ? s[t][0] * f0 : -INFINITY;
-        s[t][1] = gq < left ? s[t][1] * f1 : -INFINITY;
-        s[t][2] = gq + 8 < left ? s[t][2] * f0 : -INFINITY;
-        s[t][3] = gq + 8 < left ? s[t][3] * f1 : -INFINITY;
-        grow |= fmaxf(s[t][0], s[t][2]) > m_run[t][0] + 6.f || fmaxf(s[t][1], s[t][3]) > m_run[t][1] + 6.f;
       }
       if (left < 16) {                                          // what stands behind the last token may be anything
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (2 * tq + (r >> 1) * 8 + (r & 1) >= left)
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) x.v[r][c] = 0u;
+            for (int c = 0; c < D / 32; ++c) v[r][c] = 0u;
+      }
+      // x = score - running maximum; both of a head's tokens
+      float x[NT][4], f[NT][2];
+      bool grow = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[t][e & 1] = qs[t][e & 1] * kscale;
+          x[t][e] = fmaf(s[t][e], f[t][e & 1], -m_run[t][e & 1]);
+        }
+        if (left < 16) {
+          if (gq >= left) x[t][0] = x[t][1] = -INFINITY;
+          if (gq + 8 >= left) x[t][2] = x[t][3] = -INFINITY;
+        }
+        grow |= fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])) > 15.f;
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float m = fmaxf(s[t][e], s[t][e + 2]);
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            m = fmaxf(m, m_run[t][e]);
-            const float al = fast_exp2(m_run[t][e] - m);
-            m_run[t][e] = m;
-            l_run[t][e] *= al;
+            // from the products: the old maximum may be so far off that the difference has lost its low bits. Every lane takes
+            // part in the exchange; which heads move is the same for the eight lanes of a head only.
+            const bool in0 = gq < left, in1 = gq + 8 < left;
+            float top = fmaxf(in0 ? s[t][e] * f[t][e] : -INFINITY, in1 ? s[t][e + 2] * f[t][e] : -INFINITY);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - 9.f;              // the largest becomes 2^9
+            if (top > m_run[t][e]) {
+              const float al = fast_exp2(m_run[t][e] - top);
+              m_run[t][e] = top;
+              x[t][e] = in0 ? fmaf(s[t][e], f[t][e], -top) : -INFINITY;
+              x[t][e + 2] = in1 ? fmaf(s[t][e + 2], f[t][e], -top) : -INFINITY;
+              l_run[t][e] *= al;
 #pragma unroll
-            for (int i2 = 0; i2 < KS; ++i2) { o[t][i2][e] *= al; o[t][i2][e + 2] *= al; }
+              for (int i2 = 0; i2 < KS; ++i2) { o[t][i2][e] *= al; o[t][i2][e + 2] *= al; }
+            }
           }
       }
-      if (vscale > v_ref) {                                     // values of this page have a larger scale than those before
-        const float r = v_ref / vscale;
-        v_ref = vscale;
+      if (vscale != v_last) {                                   // another page
+        v_last = vscale;
+        if (vscale > v_ref) {                                   // whose values have a larger scale than those before
+          const float r = v_ref / vscale;
+          v_ref = vscale;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i2 = 0; i2 < KS; ++i2) { o[t][i2][0] *= r; o[t][i2][1] *= r; o[t][i2][2] *= r; o[t][i2][3] *= r; }
+            for (int i2 = 0; i2 < KS; ++i2) { o[t][i2][0] *= r; o[t][i2][1] *= r; o[t][i2][2] *= r; o[t][i2][3] *= r; }
+        }
+        const float r = v_ref > 0.f ? vscale / v_ref : 0.f;
+        ratio = pack_f16(r, r);
       }
-      const float pv = v_ref > 0.f ? vscale / v_ref * 512.f : 0.f;                  // p <= 2^6: 2^15 at most, and fp16 goes down to 2^-24
       uint32_t p0[NT], p1[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float e0 = fast_exp2(s[t][0] - m_run[t][0]), e1 = fast_exp2(s[t][1] - m_run[t][1]);
-        const float e2 = fast_exp2(s[t][2] - m_run[t][0]), e3 = fast_exp2(s[t][3] - m_run[t][1]);
+        const float e0 = fast_exp2(x[t][0]), e1 = fast_exp2(x[t][1]), e2 = fast_exp2(x[t][2]), e3 = fast_exp2(x[t][3]);
         l_run[t][0] += e0 + e2;
         l_run[t][1] += e1 + e3;
-        p0[t] = transpose8x8(pack_f16(e0 * pv, e1 * pv));
-        p1[t] = transpose8x8(pack_f16(e2 * pv, e3 * pv));
+        p0[t] = transpose8x8(mul_f16x2(pack_f16(e0, e1), ratio));
+        p1[t] = transpose8x8(mul_f16x2(pack_f16(e2, e3), ratio));
       }
 #pragma unroll
       for (int j = 0; j < KS; ++j) {                            // dims gq * D/8 + 2 j and + 2 j + 1
         const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
-        const uint32_t w0 = __byte_perm(x.v[0][j >> 1], x.v[1][j >> 1], sel), w1 = __byte_perm(x.v[2][j >> 1], x.v[3][j >> 1], sel);
+        const uint32_t w0 = __byte_perm(v[0][j >> 1], v[1][j >> 1], sel), w1 = __byte_perm(v[2][j >> 1], v[3][j >> 1], sel);
         const uint32_t a0 = half2_lo(w0), a1 = half2_hi(w0), a2 = half2_lo(w1), a3 = half2_hi(w1);
 #pragma unroll
         for (int t = 0; t < NT; ++t) mma_f16_16816(o[t][j], a0, a1, a2, a3, p0[t], p1[t]);
       }
     };
-    auto scales_of = [&]() {
-      ksc = a.ks[(size_t)pg * a.Hkv + h];
-      vsc = a.vs[(size_t)pg * a.Hkv + h];
-    };
-    if (n_tiles > 0) {
-      pg = page_of(lane);
-      scales_of();
-      pg_next = page_of(32 + lane);
-      Kv8Tile<D> x, y;
-      load(0, x);
-      for (int i = 0; i < n_tiles; i += 2) {                    // blocks of 32 tiles start at an even tile
-        if (i + 1 < n_tiles) load(i + 1, y);
-        work(i, x);
-        const float ks1 = ksc, vs1 = vsc;
-        if (i + 2 < n_tiles) {
-          if (((i + 2) & 31) == 0) {
-            pg = pg_next;
-            scales_of();
-            pg_next = page_of(i + 34 + lane);
-          }
-          load(i + 2, x);
-        }
-        if (i + 1 < n_tiles) {
-          const float ks2 = ksc, vs2 = vsc;
-          ksc = ks1; vsc = vs1;
-          work(i + 1, y);
-          ksc = ks2; vsc = vs2;
-        }
-      }
+    for (int i = 0; i < n_tiles; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+      __syncwarp();                                             // every lane's copies are here, and tile i - 1 has been read
+      fetch(i + S - 1);
+      work(i);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    float* mo = reinterpret_cast<float*>(dsm + warp * Cfg::RING);
 
     // ---- join the four warps; O^T fragments: element 0/1 = dim gq * D/8 + 2 j of heads 2 tq, 2 tq + 1; 2/3 = the next dim
-    const float unit = v_ref * (1.f / 512.f);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -516,12 +572,11 @@ kv8_decode_kernel(Kv8Decode a) {
         }
 #pragma unroll
         for (int j = 0; j < KS; ++j)
-          *reinterpret_cast<float2*>(&mo[(warp * HP + hd) * (D + 4) + gq * (D / 8) + 2 * j]) = make_float2(o[t][j][e] * unit, o[t][j][e + 2] * unit);
+          *reinterpret_cast<float2*>(&mo[hd * (D + 4) + gq * (D / 8) + 2 * j]) = make_float2(o[t][j][e] * v_ref, o[t][j][e + 2] * v_ref);
       }
     }
     __syncthreads();
-    const bool whole = c0 == 0 && c1 == nc;
-    const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+    const int slot = slots[b] * Hv + hv * np + part;
     for (int i = tid; i < ng * D; i += 128) {
       const int g = i / D, d = i - g * D;
       float mx = mm[g];
@@ -532,68 +587,77 @@ kv8_decode_kernel(Kv8Decode a) {
       for (int w = 0; w < 4; ++w) {
         const float f = fast_exp2(mm[w * HP + g] - mx);
         l += ml[w * HP + g] * f;
-        acc += mo[(w * HP + g) * (D + 4) + d] * f;
+        acc += reinterpret_cast<const float*>(dsm + w * Cfg::RING)[g * (D + 4) + d] * f;
       }
-      if (whole) {
+      if (np == 1) {
         a.out[((size_t)b * a.Hq + h * a.G + g0 + g) * D + d] = __float2bfloat16(acc / l);
       } else {
         a.part_o[((size_t)slot * HP + g) * D + d] = acc;
-        if (d == 0) {
-          a.part_ml[((size_t)slot * HP + g) * 2] = mx;
-          a.part_ml[((size_t)slot * HP + g) * 2 + 1] = l;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)slot * HP + g) * 2) = make_float2(mx, l);
+      }
+    }
+    if (np > 1) {
+      // ---- the item's last unit joins them: a warp for each head, lane i weighs part i, all lanes read its row together
+      __syncthreads();
+      if (tid == 0) {
+        __threadfence();
+        s_last = atomicInc(a.counters + 1 + b * Hv + hv, np - 1) == (unsigned)(np - 1);
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_last) {
+        const size_t first = (size_t)(slot - part) * HP;
+        constexpr int PER = D / 32;
+        for (int g = warp; g < ng; g += 4) {
+          float mx = -INFINITY, l = 0.f, acc[PER];
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+          for (int i0 = 0; i0 < np; i0 += 32) {
+            const float2 p = i0 + lane < np ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + (first + (size_t)(i0 + lane) * HP + g) * 2)) : make_float2(-INFINITY, 0.f);
+            const float m = fmaxf(mx, warp_max(p.x)), f0 = fast_exp2(mx - m), f = fast_exp2(p.x - m);
+            mx = m;
+            l = l * f0 + p.y * f;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] *= f0;
+            const float* src = a.part_o + (first + (size_t)i0 * HP + g) * D + lane * PER;
+            const int n = min(32, np - i0);
+            for (int i = 0; i < n; i += 8) {                    // eight rows on their way at a time
+              float x[8][PER];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float* p = src + (size_t)min(i + j, n - 1) * HP * D;
+                if constexpr (D == 128) *reinterpret_cast<float4*>(x[j]) = __ldcg(reinterpret_cast<const float4*>(p));
+                else *reinterpret_cast<float2*>(x[j]) = __ldcg(reinterpret_cast<const float2*>(p));
+              }
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float w = __shfl_sync(0xffffffffu, f, i + j);            // lanes behind the last part hold zero
+#pragma unroll
+                for (int e = 0; e < PER; ++e) acc[e] += x[j][e] * w;
+              }
+            }
+          }
+          const float inv = 1.f / warp_sum(l);
+          uint32_t* out = reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.Hq + h * a.G + g0 + g) * D + lane * PER);
+#pragma unroll
+          for (int e = 0; e < PER / 2; ++e) out[e] = pack_bf16(acc[2 * e] * inv, acc[2 * e + 1] * inv);
         }
       }
     }
-    if (c0 == 0 && tid == 0) {
-      // blocks that hold the item: this one to the one with its last chunk, c * grid / total rounded up as the shares are
-      int last = (int)(((item0 + nc) * grid - 1) / total);
-      a.meta[b * Hv + hv] = whole ? 0 : (slot << 10) | (last - (int)blockIdx.x);
-    }
-    __syncthreads();                                            // the buffers are free for the next segment
-    pos = item0 + c1;
-    first_segment = false;
+    if (tid == 0) s_next = (int)next;
+    __syncthreads();                                            // the buffers are free for the next unit
+    unit = s_next;
   }
-}
-
-// Joins the partial results of items that were split over blocks: the first in slot `slot`, the others in the first slot of the
-// blocks behind. A row without tokens gets zeros.
-template <int D, int NT>
-__global__ void __launch_bounds__(D) kv8_join_kernel(Kv8Decode a) {
-  constexpr int HP = 8 * NT;
-  pdl_wait();
-  pdl_trigger();
-  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq, d = threadIdx.x;
-  const int h = hq / a.G, gh = hq - h * a.G, grp = gh / 16, g = gh - grp * 16;
-  __nv_bfloat16* out = a.out + (size_t)blockIdx.x * D + d;
-  if (a.lens[b] <= 0) {
-    *out = __float2bfloat16(0.f);
-    return;
-  }
-  const int meta = a.meta[b * a.Hkv * a.groups + h * a.groups + grp];
-  if (meta == 0) return;
-  const int slot = meta >> 10, more = meta & 1023, next = (slot >> 1) + 1;
-  auto row = [&](int i) { return (size_t)(i == 0 ? slot : 2 * (next + i - 1)) * HP + g; };
-  float mx = -INFINITY;
-  for (int i = 0; i <= more; ++i) mx = fmaxf(mx, a.part_ml[row(i) * 2]);
-  float l = 0.f, acc = 0.f;
-#pragma unroll 8
-  for (int i = 0; i <= more; ++i) {
-    const float f = fast_exp2(a.part_ml[row(i) * 2] - mx);
-    l += a.part_ml[row(i) * 2 + 1] * f;
-    acc += a.part_o[row(i) * D + d] * f;
-  }
-  *out = __float2bfloat16(acc / l);
 }
 
 template <int D, int NT>
 static int launch_kv8_decode(const Kv8Decode& a, int grid, cudaStream_t s) {
-  constexpr int HP = 8 * NT;
-  const int smem = (4 * HP * (D + 4) + 8 * HP + a.B + 1) * 4;
+  constexpr int HP = 8 * NT, RING = 4 * Kv8Cfg<D, NT>::RING + 8 * HP * 4;
+  const int smem = RING + 2 * (a.B + 1) * 4;
   auto kern = kv8_decode_kernel<D, NT>;
   static ab2host::DevState st;
-  if (ab2host::prepare_launch(kern, (4 * HP * (D + 4) + 8 * HP + 8192 + 1) * 4, st, nullptr)) return 2;
+  if (ab2host::prepare_launch(kern, RING + 2 * (KV8_MOST_ROWS + 1) * 4, st, nullptr)) return 2;
   launch_pdl(kern, dim3(grid), dim3(128), (size_t)smem, s, a);
-  launch_pdl(kv8_join_kernel<D, NT>, dim3(a.B * a.Hq), dim3(D), 0, s, a);
   return cudaGetLastError() == cudaSuccess ? 0 : 1;
 }
 
@@ -703,38 +767,45 @@ int ab2_kv8_append(const void* k, const void* v, void* kc, void* vc, void* ks, v
 static int kv8_grid(int B, int Hq, int Hkv, int width, int page_size, int sms) {
   const int G = Hq / Hkv, groups = (G + 15) / 16;
   const long long most = (long long)B * Hkv * groups * (((long long)width * page_size + KV8_CHUNK - 1) / KV8_CHUNK);
-  const long long wave = (long long)sms * (G <= 8 ? 3 : 2);
+  const long long wave = (long long)sms * (G <= 8 ? Kv8Cfg<128, 1>::BLOCKS : Kv8Cfg<128, 2>::BLOCKS);
   return (int)(most < wave ? most : wave);
 }
-long long ab2_kv8_decode_workspace(int B, int Hq, int Hkv, int D, int page_size, int width) {
+// Bytes of the workspace, and in *counters the unsigned counters beside it. A split item has at least two units, so no more than
+// 2 * blocks * rounds units belong to split items.
+long long ab2_kv8_decode_workspace(int B, int Hq, int Hkv, int D, int page_size, int width, int* counters) {
   if (B <= 0 || Hkv <= 0 || Hq % Hkv) return 0;
   const int G = Hq / Hkv, groups = (G + 15) / 16, HP = G <= 8 ? 8 : 16;
-  const long long slots = 2LL * kv8_grid(B, Hq, Hkv, width, page_size, ab2_num_sms());
-  return slots * HP * (D + 2) * 4 + (long long)B * Hkv * groups * 4;
+  *counters = 1 + B * Hkv * groups;
+  const long long slots = 2LL * KV8_ROUNDS * kv8_grid(B, Hq, Hkv, width, page_size, ab2_num_sms());
+  return slots * HP * (D + 2) * 4;
 }
 
-// q [B, Hq, D] bf16 (rows q_stride elements apart, heads dense), out [B, Hq, D] dense; cache and table as above; lens [B].
+// q [B, Hq, D] bf16 (rows q_stride elements apart, heads dense), out [B, Hq, D] dense; cache and table as above; lens [B]. The counters are
+// zero before the call and after it; calls that may run at the same time must not share them or the workspace.
 int ab2_kv8_decode(const void* q, const void* kc, const void* vc, const void* ks, const void* vs, const int* table, const int* lens, void* out,
-                   void* workspace, int B, int Hq, int Hkv, int D, int page_size, int width, int num_pages, float scale, long long q_stride, void* stream) {
+                   void* workspace, void* counters, int B, int Hq, int Hkv, int D, int page_size, int width, int num_pages, float scale, long long q_stride,
+                   void* stream) {
   if (B <= 0) return 0;
   if (D != 64 && D != 128) return 11;
-  if (page_size <= 0 || page_size % 16) return 12;
-  if (Hkv <= 0 || Hq % Hkv || (q_stride & 7) || width <= 0 || num_pages <= 0 || B > 8192 || (long long)width * page_size > 0x7fffffffLL - 64) return 10;
+  if (page_size < 16 || (page_size & (page_size - 1))) return 12;
+  if (Hkv <= 0 || Hq % Hkv || (q_stride & 7) || width <= 0 || num_pages <= 0 || B > KV8_MOST_ROWS) return 10;
+  const int G = Hq / Hkv, groups = (G + 15) / 16;
+  // chunks of the whole batch are counted in 32 bits
+  if ((long long)width * page_size > 0x7fffffffLL - 64 || (long long)B * Hkv * groups * (((long long)width * page_size + 63) / 64) > 0x7fffffffLL - 65536) return 13;
   Kv8Decode a;
   const int grid = kv8_grid(B, Hq, Hkv, width, page_size, ab2_num_sms());
-  if (grid > 1023) return 13;
   a.q = (const __nv_bfloat16*)q; a.kc = (const unsigned char*)kc; a.vc = (const unsigned char*)vc;
   a.ks = (const float*)ks; a.vs = (const float*)vs; a.table = table; a.lens = lens; a.out = (__nv_bfloat16*)out;
-  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.groups = (a.G + 15) / 16;
-  a.page_size = page_size; a.width = width; a.num_pages = num_pages;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = G; a.groups = groups;
+  a.page_size = page_size; a.page_bits = __builtin_ctz(page_size); a.width = width; a.num_pages = num_pages;
   a.scale_log2 = scale * 1.4426950408889634f; a.q_stride = q_stride; a.err = ab2host::error_flag();
-  const int HP = a.G <= 8 ? 8 : 16;
+  const int HP = G <= 8 ? 8 : 16;
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + 2LL * grid * HP * D;
-  a.meta = (int*)(a.part_ml + 2LL * grid * HP * 2);
+  a.part_ml = a.part_o + 2LL * KV8_ROUNDS * grid * HP * D;
+  a.counters = (unsigned int*)counters;
   cudaStream_t s = (cudaStream_t)stream;
-  if (D == 128) return a.G <= 8 ? launch_kv8_decode<128, 1>(a, grid, s) : launch_kv8_decode<128, 2>(a, grid, s);
-  return a.G <= 8 ? launch_kv8_decode<64, 1>(a, grid, s) : launch_kv8_decode<64, 2>(a, grid, s);
+  if (D == 128) return G <= 8 ? launch_kv8_decode<128, 1>(a, grid, s) : launch_kv8_decode<128, 2>(a, grid, s);
+  return G <= 8 ? launch_kv8_decode<64, 1>(a, grid, s) : launch_kv8_decode<64, 2>(a, grid, s);
 }
 
 // n_buf buffers, each ten values in `desc`: address, plane, page and row strides in bytes, planes, rows, bytes of a row, bytes of a token in a

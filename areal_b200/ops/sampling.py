@@ -62,25 +62,29 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, inv_temp: torch.Tenso
 
     ``u``, ``inv_temp``, ``top_p``, ``min_p``: fp32 ``[B]``; ``top_k``, ``greedy``: int32 ``[B]``. Rows of logits may lie apart (a slice of a wider
     tensor). At most 393216 tokens in the vocabulary on CUDA."""
-    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits: fp32 [B, V], dense rows")
-    B, V = logits.shape
-    dev = logits.device
+    shape = logits.shape
+    if not (len(shape) == 2 and logits.dtype is torch.float32 and shape[1] > 0 and (logits.stride(1) == 1 or shape[1] == 1)):
+        raise ValueError("logits: fp32 [B, V], dense rows")
+    B, V = shape
+    dev, one = logits.get_device(), shape[:1]
     for t, d, name in ((u, torch.float32, "u"), (inv_temp, torch.float32, "inv_temp"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"),
                        (top_k, torch.int32, "top_k"), (greedy, torch.int32, "greedy")):
-        if t is not None:
-            _need(t.dtype == d and t.shape == (B,) and t.is_contiguous() and t.device == dev, f"{name}: contiguous {d} [{B}] beside the logits")
+        if t is not None and not (t.dtype is d and t.shape == one and t.is_contiguous() and t.get_device() == dev):
+            raise ValueError(f"{name}: contiguous {d} [{B}] beside the logits")
     if out is not None:
-        _need(out[0].dtype == torch.int32 and out[1].dtype == torch.float32 and all(t.shape == (B,) and t.is_contiguous() and t.device == dev for t in out),
+        _need(out[0].dtype == torch.int32 and out[1].dtype == torch.float32 and all(t.shape == one and t.is_contiguous() and t.get_device() == dev for t in out),
               "out: int32 and fp32, contiguous [B]")
-    if not logits.is_cuda:
+    if dev < 0:
         r = sample_filtered_ref(logits, u, inv_temp, top_k, top_p, min_p, greedy)
         return r if out is None else (out[0].copy_(r[0]), out[1].copy_(r[1]))
-    _need(V <= MAX_VOCAB, f"a vocabulary of {V}: at most {MAX_VOCAB}")
+    if V > MAX_VOCAB:
+        raise ValueError(f"a vocabulary of {V}: at most {MAX_VOCAB}")
     ld = logits.stride(0) if B > 1 else V
-    _need(ld >= V, "rows of logits overlap")
+    if ld < V:
+        raise ValueError("rows of logits overlap")
     if out is None:
-        out = torch.empty(B, dtype=torch.int32, device=dev), torch.empty(B, device=dev)
-    _launch(logits, "ab2_sample_filtered", logits.data_ptr(), ld, B, V, u.data_ptr(), inv_temp.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+        out = torch.empty(B, dtype=torch.int32, device=logits.device), torch.empty(B, device=logits.device)
+    _launch(dev, "ab2_sample_filtered", logits.data_ptr(), ld, B, V, u.data_ptr(), inv_temp.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
             min_p.data_ptr(), None if greedy is None else greedy.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
     return out
 
