@@ -14,6 +14,8 @@
 // tokens of a usual row), which sorts it and finishes alone. A nucleus of more than 2048 tokens: only the undecided bins go
 // to the list, the first block gives the last kept value and how many tokens with that value are kept, and the blocks then sum
 // their kept weights by index. Where even the undecided bins are too full (thousands of equal logits), the range is cut again.
+#include <cmath>
+
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -24,7 +26,9 @@ namespace cg = cooperative_groups;
 constexpr int SF_THREADS = 512, SF_WARPS = SF_THREADS / 32;
 constexpr int SF_BINS = 2048;          // four for each thread
 constexpr int SF_CAP = 2048;           // entries of the list
-constexpr int SF_SEGS = 128;           // pieces of a block's share with sums of their own, eight for each warp
+constexpr int SF_SEG = 256;            // logits of a piece of a block's share that has a sum of its own
+constexpr int SF_SEGS = 200;           // at most
+constexpr float SF_FAR = 16.6f;        // nats below the maximum from where single precision will do for a total (2^-24 of the maximum)
 constexpr int SF_MAX_CLUSTER = 8;
 constexpr float SF_PER_NAT = 64.f;
 
@@ -37,12 +41,14 @@ struct SampleArgs {
   float* out_logp;
   int V, share;                        // share: logits of one block, a multiple of 4
   int aligned;                         // rows start on 16 bytes
+  int index_shift;                     // index >> index_shift numbers at most SF_BINS buckets
+  double tab[32];                      // 2^(j/32)
 };
 
 struct SampleShared {
   unsigned long long list[SF_CAP];
   unsigned int hist[SF_BINS];
-  double tab[64];                      // 2^(j/64)
+  double tab[32];                      // 2^(j/32): the entries of a half warp fall on banks of their own
   double seg_sum[SF_SEGS];
   int seg_tie[SF_SEGS];
   // what the blocks of the cluster tell one another; two sets in turn, since a fast block may write the next before a slow one has read
@@ -56,20 +62,20 @@ struct SampleShared {
   int ties, list_n, cut[4];
 };
 
-// exp(d) for d <= 0 in 64 bits: exp(d) = 2^k * 2^(j/64) * exp(r), |r| <= ln 2 / 128, the last by its Taylor polynomial (table-driven
-// exponentials after P. T. P. Tang, 1989; relative error below 5e-14). Zero below e^-700.
+// exp(d) for d <= 0 in 64 bits: exp(d) = 2^k * 2^(j/32) * exp(r), |r| <= ln 2 / 64, the last by its Taylor polynomial (table-driven
+// exponentials after P. T. P. Tang, 1989; relative error below 2e-12). Zero below e^-700.
 __device__ __forceinline__ double weight(double d, const double* tab) {
-  if (!(d >= -700.0)) return 0.0;
   const double big = 6755399441055744.0;                       // 1.5 * 2^52: adding it rounds to a whole number
-  const double t = fma(d, 92.332482616893656877, big);         // 64 / ln 2
+  const double t = fma(d, 46.166241308446828, big);            // 32 / ln 2
   const int k = __double2loint(t);
-  const double r = fma(t - big, -0.010830424696249145, d);     // ln 2 / 64
+  const double r = fma(t - big, -0.021660849392498290, d);     // ln 2 / 32
   double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
   p = fma(p, r, 0.5);
   p = fma(p, r, 1.0);
   p = fma(p, r, 1.0);
-  const double w = p * tab[k & 63];
-  return __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
+  const double w = p * tab[k & 31];
+  const double v = __hiloint2double(__double2hiint(w) + ((k >> 5) << 20), __double2loint(w));
+  return d >= -700.0 ? v : 0.0;
 }
 // Order-preserving map of floats to unsigned.
 __device__ __forceinline__ unsigned int key_of(float x) {
@@ -112,6 +118,41 @@ __device__ __forceinline__ int pow2_above(int n) {
   return p;
 }
 
+// Sorts list[0 .. n) falling, n <= SF_CAP, given each entry's bucket (rising as the keys fall) and end[b] = entries of the buckets before b on
+// entry: an entry goes behind what its bucket holds already, and then to its rank among the few of its bucket. Keys are all different.
+template <typename F>
+__device__ __forceinline__ void sort_buckets(unsigned long long* list, int n, unsigned int* end, F bucket) {
+  unsigned long long e[SF_CAP / SF_THREADS];
+  int at[SF_CAP / SF_THREADS];
+#pragma unroll
+  for (int j = 0; j < SF_CAP / SF_THREADS; ++j) {
+    const int i = threadIdx.x + j * SF_THREADS;
+    if (i < n) {
+      e[j] = list[i];
+      at[j] = atomicAdd(&end[bucket(e[j])], 1u);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < SF_CAP / SF_THREADS; ++j)
+    if ((int)threadIdx.x + j * SF_THREADS < n) list[at[j]] = e[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < SF_CAP / SF_THREADS; ++j)
+    if ((int)threadIdx.x + j * SF_THREADS < n) {
+      const int b = bucket(e[j]), last = end[b];
+      const int from = b > 0 ? end[b - 1] : 0;
+      int r = from;
+      for (int i = from; i < last; ++i) r += list[i] > e[j];
+      at[j] = r;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < SF_CAP / SF_THREADS; ++j)
+    if ((int)threadIdx.x + j * SF_THREADS < n) list[at[j]] = e[j];
+  __syncthreads();
+}
+
 // Sum over the block of each thread's value before this thread (exclusive, in thread order), and the total.
 __device__ __forceinline__ double block_scan(double v, double* red, double* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -125,6 +166,26 @@ __device__ __forceinline__ double block_scan(double v, double* red, double* tota
   if (lane == 31) red[warp] = s;
   __syncthreads();
   double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int w = 0; w < SF_WARPS; ++w) {
+    if (w == warp) before = all;
+    all += red[w];
+  }
+  *total = all;
+  return before + (s - v);
+}
+__device__ __forceinline__ float block_scan_f(float v, float* red, float* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = s;
+  __syncthreads();
+  float before = 0.f, all = 0.f;
 #pragma unroll
   for (int w = 0; w < SF_WARPS; ++w) {
     if (w == warp) before = all;
@@ -195,9 +256,10 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     } else {
       for (int i = tid; i < n; i += SF_THREADS) { const float v = clean(src[i]); xs[i] = v; mx = fmaxf(mx, v); }
     }
+    for (int i = max(n, 0) + tid; i < a.share; i += SF_THREADS) xs[i] = -INFINITY;
   }
   for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
-  if (tid < 64) sh.tab[tid] = exp2(tid * (1.0 / 64.0));
+  if (tid < 32) sh.tab[tid] = a.tab[tid];
   if (tid == 0) sh.list_n = 0;
   mx = warp_max(mx);
   if (lane == 0) sh.fred[0][warp] = mx;
@@ -282,8 +344,315 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   float thr = -INFINITY;                // kept: x > thr, and the first `ties` (by index) of those equal to it
   int ties = 0;
   double total = 0.0;                   // what top_p is a share of
-  // by count first (top-k), then by mass (top-p), each only where asked for; min-p alone goes through once to try for the list
-  for (int stage = 0; stage < 2; ++stage) {
+  // The list holds, in order, everything that can be kept: what of it is, and the token.
+  auto finish = [&](int cnt) {
+    const int k = K > 0 ? min(K, cnt) : cnt;
+    double w[4], mine = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = 4 * tid + j;
+      w[j] = i < k ? w_of(float_of((unsigned int)(sh.list[i] >> 32))) : 0.0;
+      mine += w[j];
+    }
+    double sum;
+    double run = block_scan(mine, sh.red, &sum);
+    const double all = K > 0 ? sum : total;
+    int kept = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = 4 * tid + j;
+      if (i < k && w[j] > 0.0 && (!by_mass || run <= top_p * all) && w[j] >= min_p) ++kept;
+      run += w[j];
+    }
+    int m;
+    block_scan_i(kept, sh.ired, &m);
+    if (m == 0) m = 1;
+    // the kept ones by index: the key's low half, the index's complement, to the front
+    for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
+    __syncthreads();
+    auto bucket = [&](unsigned long long e) { return (int)((0xffffffffu - (unsigned int)(e >> 32)) >> a.index_shift); };
+    for (int i = tid; i < m; i += SF_THREADS) {
+      const unsigned long long e = (sh.list[i] << 32) | (sh.list[i] >> 32);
+      sh.list[i] = e;
+      atomicAdd(&sh.hist[bucket(e)], 1u);
+    }
+    __syncthreads();
+    const uint4 c = reinterpret_cast<const uint4*>(sh.hist)[tid];
+    int all_i;
+    const unsigned int at = block_scan_i((int)(c.x + c.y + c.z + c.w), sh.ired, &all_i);
+    reinterpret_cast<uint4*>(sh.hist)[tid] = make_uint4(at, at + c.x, at + c.x + c.y, at + c.x + c.y + c.z);
+    __syncthreads();
+    sort_buckets(sh.list, m, sh.hist, bucket);
+    mine = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = 4 * tid + j;
+      w[j] = i < m ? w_of(float_of((unsigned int)sh.list[i])) : 0.0;
+      mine += w[j];
+    }
+    run = block_scan(mine, sh.red, &sum);
+    const double goal = fmax((double)a.u[row], 0.0) * sum;
+    int hit = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      run += w[j];
+      if (4 * tid + j < m && run > goal) hit = min(hit, 4 * tid + j);
+    }
+    hit = __reduce_min_sync(0xffffffffu, hit);
+    __syncthreads();
+    if (lane == 0) sh.ired[warp] = hit;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w2 = 1; w2 < SF_WARPS; ++w2) hit = min(hit, sh.ired[w2]);
+      if (hit >= m) hit = m - 1;
+      const unsigned long long v = sh.list[hit];
+      a.out_tok[row] = (int)(0xffffffffu - (unsigned int)(v >> 32));
+      a.out_logp[row] = (float)log(w_of(float_of((unsigned int)v)) / sum);
+    }
+  };
+
+  // ---- the usual way: one histogram of the whole row, one look at what the border needs
+  const int n4 = a.share / 4, segs = (a.share + SF_SEG - 1) / SF_SEG;
+  const float4* xs4 = reinterpret_cast<const float4*>(xs);
+  bool decided = !(K > 0 || by_mass || by_min);         // thr and ties are known
+  bool summed = false;                                   // seg_sum has the weights of what is before t_sure
+  float t_sure = 0.f;                                    // in bins below the maximum: what is before is kept, whatever thr is
+  const float scale = itf * SF_PER_NAT;
+  if (!decided) {
+    {
+      double s = 0.0;
+      float far = 0.f;
+      int behind = 0;
+#pragma unroll 2
+      for (int i = tid; i < n4; i += SF_THREADS) {
+        const float4 v = xs4[i];
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        float t[4];
+        bool near = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          t[j] = (xmax - x[j]) * scale;
+          near |= t[j] < SF_FAR * SF_PER_NAT;
+        }
+        if (by_mass && K == 0) {
+          if (near) {
+            double w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = weight(((double)x[j] - top) * it, sh.tab);
+            s += (w[0] + w[1]) + (w[2] + w[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) far += fast_exp2(t[j] * (-1.4426950408889634f / SF_PER_NAT));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (t[j] < (float)(SF_BINS - 1)) atomicAdd(&sh.hist[(int)t[j]], 1u);
+          else if (x[j] > -INFINITY) ++behind;
+        }
+      }
+      behind = warp_sum_i(behind);
+      if (lane == 0 && behind) atomicAdd(&sh.hist[SF_BINS - 1], (unsigned int)behind);
+      if (by_mass && K == 0) publish_sum(s + (double)far);
+    }
+    cl.sync();
+    if (by_mass && K == 0) { total = all_sum(); buf ^= 1; }
+    unsigned int c[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 8
+    for (int i = 0; i < nb; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(cl.map_shared_rank(sh.hist, i))[tid];
+      c[0] += v.x; c[1] += v.y; c[2] += v.z; c[3] += v.w;
+    }
+    int c_total;
+    const int c_before = block_scan_i((int)(c[0] + c[1] + c[2] + c[3]), sh.ired, &c_total);
+    K = min(K, c_total);                                                          // no more tokens than that have any weight
+    if (tid == 0) { sh.cut[0] = SF_BINS; sh.cut[1] = SF_BINS; sh.cut[2] = c_total; sh.cut[3] = 0; }
+    __syncthreads();
+    if (K > 0) {
+      int at = c_before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (at < K && at + (int)c[j] >= K) { sh.cut[0] = 0; sh.cut[1] = 4 * tid + j; sh.cut[2] = at + (int)c[j]; sh.cut[3] = 0; }
+        at += (int)c[j];
+      }
+    } else if (by_mass && total > 0.0) {
+      // a bin's weights lie between those of its edges, exp(-b / 64) and exp(-(b + 1) / 64), but for the open last one: from those, bounds
+      // on what is before and behind a bin's end. Single precision, and the rounding of x to its bin, stay well within `slack`.
+      const float f = 0.98449643700540842f, slack = 4e-5f;                        // exp(-1 / 64)
+      const float w0 = fast_exp2(tid * (-4.f * 1.4426950408889634f / SF_PER_NAT));
+      float lo[4], m = 0.f, e = w0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        e *= f;
+        lo[j] = 4 * tid + j < SF_BINS - 1 ? (float)c[j] * e : 0.f;
+        m += lo[j];
+      }
+      float m_all;
+      float m_cum = block_scan_f(m, sh.fred[0], &m_all);
+      if (tid == SF_THREADS - 1) sh.fred[1][0] = (float)c[3] * e / f;
+      __syncthreads();
+      const float last_hi = sh.fred[1][0], want = (float)(top_p * total), rest = (float)(total - top_p * total);
+      int at = c_before, b1 = SF_BINS, b2 = SF_BINS, c1 = 0, c2 = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m_cum += lo[j];
+        const bool end = 4 * tid + j == SF_BINS - 1;
+        const float behind = fmaxf(m_all - m_cum, 0.f), fuzz = slack * m_all;     // the difference of two sums is off by a part of them
+        const bool maybe = c[j] && (end || (m_cum / f * (1.f + slack) > want && (behind - fuzz) * (1.f - slack) < rest));
+        const bool sure = c[j] && (end || m_cum * (1.f - slack) > want || ((behind + fuzz) / f + last_hi) * (1.f + slack) < rest);
+        if (maybe && b1 == SF_BINS) { b1 = 4 * tid + j; c1 = at; }
+        at += (int)c[j];
+        if (sure && b2 == SF_BINS) { b2 = 4 * tid + j; c2 = at; }
+      }
+      if (b1 < SF_BINS) atomicMin(&sh.cut[0], b1);
+      if (b2 < SF_BINS) atomicMin(&sh.cut[1], b2);
+      __syncthreads();
+      if (b1 < SF_BINS && sh.cut[0] == b1) sh.cut[3] = c1;
+      if (b2 < SF_BINS && sh.cut[1] == b2) sh.cut[2] = c2;
+    } else if (by_min) {
+      // ln(1 / min_p) below the maximum, a bin further for what rounding does to the edges
+      const double t = -log(min_p) * (double)SF_PER_NAT + 1.0;
+      const int b2 = t < (double)(SF_BINS - 1) ? (int)t : SF_BINS - 1;
+      if (tid == b2 >> 2) {
+        int at = c_before;
+        for (int j = 0; j <= (b2 & 3); ++j) at += (int)c[j];
+        sh.cut[0] = 0; sh.cut[1] = b2; sh.cut[2] = at; sh.cut[3] = 0;
+      }
+    }
+    __syncthreads();
+    int b1 = sh.cut[0], b2 = sh.cut[1], before = sh.cut[3];
+    const int upto = sh.cut[2];
+    if (b2 >= SF_BINS) b2 = SF_BINS - 1;
+    if (b1 > b2) b1 = before = 0;
+    const bool whole = upto <= SF_CAP, part = !whole && K == 0 && by_mass && upto - before <= SF_CAP;
+    if (whole || part) {
+      const bool to_end = b2 == SF_BINS - 1;
+      const float t_list = (float)(b2 + 1);
+      t_sure = whole ? 0.f : (float)b1;
+      SampleShared* head = cl.map_shared_rank(&sh, 0);
+      for (int g = warp; g < segs; g += SF_WARPS) {
+        double s = 0.0;
+#pragma unroll
+        for (int h = 0; h < SF_SEG / 128; ++h) {
+          const int i = g * (SF_SEG / 4) + h * 32 + lane;
+          const float4 v = i < n4 ? xs4[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          const float x[4] = {v.x, v.y, v.z, v.w};
+          float t[4];
+          bool some = to_end, sure = false;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            t[j] = (xmax - x[j]) * scale;
+            some |= t[j] < t_list;
+            sure |= t[j] < t_sure;
+          }
+          if (sure) {
+            double w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = t[j] < t_sure ? weight(((double)x[j] - top) * it, sh.tab) : 0.0;
+            s += (w[0] + w[1]) + (w[2] + w[3]);
+          }
+          if (__any_sync(0xffffffffu, some)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool take = (to_end || t[j] < t_list) && !(t[j] < t_sure) && x[j] > -INFINITY;
+              const unsigned int who = __ballot_sync(0xffffffffu, take);
+              if (who) {
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&sh.list_n, __popc(who));
+                at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+                if (take && at < SF_CAP) sh.list[at] = ((unsigned long long)key_of(x[j]) << 32) | (0xffffffffu - (unsigned int)(begin + 4 * i + j));
+              }
+            }
+          }
+        }
+        if (part) {
+          s = warp_sum_d(s);
+          if (lane == 0) sh.seg_sum[g] = s;
+        }
+      }
+      __syncthreads();
+      if (me != 0) {                                                              // the first block's list takes them all
+        const int k = sh.list_n;
+        if (tid == 0 && k) sh.ired[0] = atomicAdd(&head->list_n, k);
+        __syncthreads();
+        const int at = sh.ired[0];
+        for (int i = tid; i < k && at + i < SF_CAP; i += SF_THREADS) head->list[at + i] = sh.list[i];
+      }
+      if (part) {
+        double s = 0.0;
+        for (int g = tid; g < segs; g += SF_THREADS) s += sh.seg_sum[g];
+        publish_sum(s);
+      }
+      cl.sync();
+      if (whole && me != 0) return;
+      int cnt = 0;
+      if (me == 0) {
+        cnt = min(sh.list_n, SF_CAP);
+        unsigned int at = c_before - (whole ? 0 : before);
+        uint4 e;
+        e.x = at; e.y = at += c[0]; e.z = at += c[1]; e.w = at += c[2];
+        reinterpret_cast<uint4*>(sh.hist)[tid] = e;                               // entries of the list before each bin (of those in it)
+        __syncthreads();
+        if (tid == 0 && b1 > 0 && !whole) sh.hist[b1 - 1] = 0u;
+        __syncthreads();
+        sort_buckets(sh.list, cnt, sh.hist, [&](unsigned long long q) { return (int)fminf((xmax - float_of((unsigned int)(q >> 32))) * scale, (float)(SF_BINS - 1)); });
+      }
+      if (whole) {
+        finish(cnt);
+        return;
+      }
+      const double s_above = all_sum();
+      buf ^= 1;
+      if (me == 0) {
+        double w[4], mine = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * tid + j;
+          w[j] = i < cnt ? w_of(float_of((unsigned int)(sh.list[i] >> 32))) : 0.0;
+          mine += w[j];
+        }
+        double sum;
+        double run = s_above + block_scan(mine, sh.red, &sum);
+        int kept = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (4 * tid + j < cnt && run <= top_p * total) ++kept;
+          run += w[j];
+        }
+        int m;
+        block_scan_i(kept, sh.ired, &m);
+        const unsigned int last = m > 0 ? (unsigned int)(sh.list[m - 1] >> 32) : 0u;
+        int same = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * tid + j < m && (unsigned int)(sh.list[4 * tid + j] >> 32) == last) ++same;
+        int eq;
+        block_scan_i(same, sh.ired, &eq);
+        if (tid < nb) {
+          SampleShared* o = cl.map_shared_rank(&sh, tid);
+          // nothing of the list kept (the border at its very start): what is above it, up to the lowest value that is
+          o->thr = m > 0 ? float_of(last) : INFINITY;
+          o->ties = eq;
+        }
+      }
+      cl.sync();
+      thr = sh.thr;
+      ties = sh.ties;
+      decided = true;
+      summed = !by_min;                                                           // min-p may take some of those away
+    } else if (K == 0 && !by_mass) {
+      decided = true;                                                             // min-p alone: every token is looked at anyway
+    }
+    if (!decided) {
+      cl.sync();                                                                  // every block has read the histograms
+      for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
+      if (tid == 0) sh.list_n = 0;
+      __syncthreads();
+    }
+  }
+
+  // ---- where that did not do (a top-k beyond the list, or thousands of tokens in the undecided bins): by count first, then by mass
+  for (int stage = 0; stage < 2 && !decided; ++stage) {
     const bool counting = stage == 0 && K > 0;
     const bool mass = stage == 1 && by_mass;
     const bool min_only = stage == 1 && !by_mass && by_min && K == 0;
@@ -449,76 +818,12 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       }
       cl.sync();
       if (whole) {
-        // ---- everything that can be kept is in the first block's list
         if (me != 0) return;
         const int cnt = min(sh.list_n, SF_CAP), n2 = pow2_above(cnt);
         for (int i = cnt + tid; i < n2; i += SF_THREADS) sh.list[i] = 0ull;
         __syncthreads();
         sort_falling(sh.list, n2);
-        const int k = K > 0 ? min(K, cnt) : cnt;
-        double w[4], mine = 0.0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 4 * tid + j;
-          w[j] = i < k ? w_of(float_of((unsigned int)(sh.list[i] >> 32))) : 0.0;
-          mine += w[j];
-        }
-        double sum;
-        double run = block_scan(mine, sh.red, &sum);
-        const double all = K > 0 ? sum : total;
-        int kept = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 4 * tid + j;
-          if (i < k && w[j] > 0.0 && (!by_mass || run <= top_p * all) && w[j] >= min_p) ++kept;
-          run += w[j];
-        }
-        int m;
-        block_scan_i(kept, sh.ired, &m);
-        if (m == 0) m = 1;
-        // the kept ones by index
-        const int m2 = pow2_above(m);
-        __syncthreads();
-        unsigned long long e[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = tid + j * SF_THREADS;
-          e[j] = i < m ? sh.list[i] : 0ull;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = tid + j * SF_THREADS;
-          if (i < m2) sh.list[i] = i < m ? (e[j] << 32) | (e[j] >> 32) : 0ull;    // high half: ~index, falling = index rising
-        }
-        __syncthreads();
-        sort_falling(sh.list, m2);
-        mine = 0.0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 4 * tid + j;
-          w[j] = i < m ? w_of(float_of((unsigned int)sh.list[i])) : 0.0;
-          mine += w[j];
-        }
-        run = block_scan(mine, sh.red, &sum);
-        const double goal = fmax((double)a.u[row], 0.0) * sum;
-        int hit = 0x7fffffff;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          run += w[j];
-          if (4 * tid + j < m && run > goal) hit = min(hit, 4 * tid + j);
-        }
-        hit = __reduce_min_sync(0xffffffffu, hit);
-        __syncthreads();
-        if (lane == 0) sh.ired[warp] = hit;
-        __syncthreads();
-        if (tid == 0) {
-          for (int w2 = 1; w2 < SF_WARPS; ++w2) hit = min(hit, sh.ired[w2]);
-          if (hit >= m) hit = m - 1;
-          const unsigned long long v = sh.list[hit];
-          a.out_tok[row] = (int)(0xffffffffu - (unsigned int)(v >> 32));
-          a.out_logp[row] = (float)log(w_of(float_of((unsigned int)v)) / sum);
-        }
+        finish(cnt);
         return;
       }
       if (mass) s_above += all_sum();
@@ -626,23 +931,38 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   }
 
   // ---- kept weights summed by index: pieces of the block's share, blocks, row
-  const int len = (a.share + SF_SEGS * 32 - 1) / (SF_SEGS * 32) * 32;             // logits of a piece
-  for (int q = 0; q < SF_SEGS / SF_WARPS; ++q) {
-    const int sg = warp * (SF_SEGS / SF_WARPS) + q;
+  for (int g = warp; g < segs; g += SF_WARPS) {
     double s = 0.0;
     int eq = 0;
-    for (int i = sg * len + lane; i < min(n, (sg + 1) * len); i += 32) {
-      const float x = xs[i];
-      if (x > thr) {
-        const double w = w_of(x);
-        if (w >= min_p) s += w;
-      } else if (x == thr && x != -INFINITY) {
-        ++eq;
+    bool some = false;
+#pragma unroll
+    for (int h = 0; h < SF_SEG / 128; ++h) {
+      const int i = g * (SF_SEG / 4) + h * 32 + lane;
+      const float4 v = i < n4 ? xs4[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      double w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool sure = (xmax - x[j]) * scale < t_sure;
+        const bool new_one = summed ? x[j] > thr && !sure : x[j] > thr || sure;
+        w[j] = 0.0;
+        if (new_one) {
+          w[j] = w_of(x[j]);
+          some = true;
+        }
+        if (w[j] < min_p) w[j] = 0.0;
+        if (x[j] == thr && x[j] != -INFINITY) { ++eq; some = true; }
       }
+      s += (w[0] + w[1]) + (w[2] + w[3]);
     }
-    s = warp_sum_d(s);
-    eq = warp_sum_i(eq);
-    if (lane == 0) { sh.seg_sum[sg] = s; sh.seg_tie[sg] = eq; }
+    if (!summed || __any_sync(0xffffffffu, some)) {
+      s = warp_sum_d(s);
+      eq = warp_sum_i(eq);
+    }
+    if (lane == 0) {
+      sh.seg_sum[g] = summed ? sh.seg_sum[g] + s : s;
+      sh.seg_tie[g] = eq;
+    }
   }
   __syncthreads();
   double w_tie = thr == -INFINITY ? 0.0 : w_of(thr);
@@ -650,8 +970,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   if (warp == 0) {
     double s = 0.0;
     int eq = 0;
-#pragma unroll
-    for (int j = 0; j < SF_SEGS / 32; ++j) { s += sh.seg_sum[lane * (SF_SEGS / 32) + j]; eq += sh.seg_tie[lane * (SF_SEGS / 32) + j]; }
+    for (int g = lane; g < segs; g += 32) { s += sh.seg_sum[g]; eq += sh.seg_tie[g]; }
     s = warp_sum_d(s);
     eq = warp_sum_i(eq);
     if (lane < nb) {
@@ -675,28 +994,47 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   // the first block whose end passes the goal (the last one with any weight, should rounding leave none)
   const bool mine = my_sum > 0.0 && my_begin <= goal && (my_begin + my_sum > goal || me == last);
   if (!mine || warp != 0) return;
-  double run = my_begin;
+  // the piece: 32 at a time, lane by lane
+  double run = my_begin, sg_run = 0.0;
   int left = my_ties, sg = -1, sg_left = 0;
-  double sg_run = 0.0;
-  for (int i = 0; i < SF_SEGS; ++i) {                                             // every lane the same
-    const int t = min(sh.seg_tie[i], left);
-    const double s = sh.seg_sum[i] + t * w_tie;
-    if (s > 0.0) { sg = i; sg_run = run; sg_left = left; }
-    run += s;
-    left -= t;
-    if (s > 0.0 && run > goal) break;
+  for (int g0 = 0; g0 < segs; g0 += 32) {
+    const int g = g0 + lane, eq = g < segs ? sh.seg_tie[g] : 0;
+    int before = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += t;
+    }
+    const int here = max(0, min(eq, left - (before - eq)));
+    const double own = (g < segs ? sh.seg_sum[g] : 0.0) + here * w_tie;
+    double s = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += t;
+    }
+    const unsigned int some = __ballot_sync(0xffffffffu, own > 0.0), hit = __ballot_sync(0xffffffffu, own > 0.0 && run + s > goal);
+    if (some) {
+      const int from = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+      sg = g0 + from;
+      sg_run = run + __shfl_sync(0xffffffffu, s - own, from);
+      sg_left = max(0, left - __shfl_sync(0xffffffffu, before - eq, from));
+    }
+    if (hit) break;
+    run += __shfl_sync(0xffffffffu, s, 31);
+    left = max(0, left - __shfl_sync(0xffffffffu, before, 31));
   }
   int tok = -1;
   double w_tok = 0.0;
   run = sg_run;
   left = sg_left;
-  for (int i0 = sg * len; i0 < min(n, (sg + 1) * len); i0 += 32) {
+  for (int i0 = sg * SF_SEG; i0 < min(a.share, (sg + 1) * SF_SEG); i0 += 32) {
     const int i = i0 + lane;
-    const float x = i < min(n, (sg + 1) * len) ? xs[i] : -INFINITY;
+    const float x = i < a.share ? xs[i] : -INFINITY;
     const unsigned int eq = __ballot_sync(0xffffffffu, x == thr && x != -INFINITY);
     const int rank = __popc(eq & ((1u << lane) - 1u));
     double w = 0.0;
-    if (x > thr) { w = w_of(x); if (w < min_p) w = 0.0; }
+    if (x > thr || (xmax - x) * scale < t_sure) { w = w_of(x); if (w < min_p) w = 0.0; }
     else if ((eq >> lane & 1u) && rank < left) w = w_tie;
     double s = w;
 #pragma unroll
@@ -736,11 +1074,14 @@ int ab2_sample_filtered(const void* logits, long long ld, int B, int V, const vo
   SampleArgs a;
   a.share = ((V + nb - 1) / nb + 3) / 4 * 4;
   const int head = (int)((sizeof(SampleShared) + 15) / 16 * 16), smem = head + a.share * 4;
-  if (smem > 227 * 1024) return 11;
+  if (smem > 227 * 1024 || a.share > SF_SEG * SF_SEGS) return 11;
   if ((long long)B * nb > 0x7fffffffLL) return 10;
   a.logits = (const float*)logits; a.ld = ld; a.u = (const float*)u; a.inv_temp = (const float*)inv_temp; a.top_p = (const float*)top_p;
   a.min_p = (const float*)min_p; a.top_k = top_k; a.greedy = greedy; a.out_tok = out_tok; a.out_logp = out_logp; a.V = V;
   a.aligned = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
+  a.index_shift = 0;
+  while ((V - 1) >> a.index_shift >= SF_BINS) ++a.index_shift;
+  for (int j = 0; j < 32; ++j) a.tab[j] = exp2(j / 32.0);
   static ab2host::DevState st;
   if (ab2host::prepare_launch(sample_filtered_kernel, 227 * 1024, st, nullptr)) return 2;
   cudaLaunchConfig_t cfg = {};
