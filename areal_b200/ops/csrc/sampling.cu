@@ -48,6 +48,7 @@ struct SampleArgs {
 struct SampleShared {
   unsigned long long list[SF_CAP];
   unsigned int hist[SF_BINS];
+  uint2 hist16[SF_BINS / 4];           // the same in 16 bits, for the other blocks (a share is below 65536)
   double tab[32];                      // 2^(j/32): the entries of a half warp fall on banks of their own
   double seg_sum[SF_SEGS];
   int seg_tie[SF_SEGS];
@@ -74,8 +75,14 @@ __device__ __forceinline__ double weight(double d, const double* tab) {
   p = fma(p, r, 1.0);
   p = fma(p, r, 1.0);
   const double w = p * tab[k & 31];
-  const double v = __hiloint2double(__double2hiint(w) + ((k >> 5) << 20), __double2loint(w));
-  return d >= -700.0 ? v : 0.0;
+  // e^-700 and less (the high word of a negative number rises as it falls; minus infinity and NaN are above them all): zero
+  const bool gone = (unsigned int)__double2hiint(d) > 0xc085e000u;
+  return __hiloint2double(gone ? 0 : __double2hiint(w) + ((k >> 5) << 20), gone ? 0 : __double2loint(w));
+}
+// float -> double by its bits, off the 64-bit pipe. Denormal numbers come out as ones of their order; infinities as +-2^128.
+__device__ __forceinline__ double widen(float x) {
+  const unsigned int b = __float_as_uint(x);
+  return __hiloint2double((int)(((b & 0x7fffffffu) >> 3) + 0x38000000u | (b & 0x80000000u)), (int)(b << 29));
 }
 // Order-preserving map of floats to unsigned.
 __device__ __forceinline__ unsigned int key_of(float x) {
@@ -120,7 +127,8 @@ __device__ __forceinline__ int pow2_above(int n) {
 
 // Sorts list[0 .. n) falling, n <= SF_CAP, given each entry's bucket (rising as the keys fall) and end[b] = entries of the buckets before b on
 // entry: an entry goes behind what its bucket holds already, and then to its rank among the few of its bucket. Keys are all different.
-template <typename F>
+// With VALUES the order of equal values (the keys' high halves) is left open, and a bucket of one value is left alone.
+template <bool VALUES = false, typename F>
 __device__ __forceinline__ void sort_buckets(unsigned long long* list, int n, unsigned int* end, F bucket) {
   unsigned long long e[SF_CAP / SF_THREADS];
   int at[SF_CAP / SF_THREADS];
@@ -140,13 +148,32 @@ __device__ __forceinline__ void sort_buckets(unsigned long long* list, int n, un
 #pragma unroll
   for (int j = 0; j < SF_CAP / SF_THREADS; ++j)
     if ((int)threadIdx.x + j * SF_THREADS < n) {
-      const int b = bucket(e[j]), last = end[b];
-      const int from = b > 0 ? end[b - 1] : 0;
-      int r = from;
-      for (int i = from; i < last; ++i) r += list[i] > e[j];
-      at[j] = r;
+      const int b = bucket(e[j]), last = (int)(end[b] & 0xffffu);
+      const int from = b > 0 ? (int)(end[b - 1] & 0xffffu) : 0;
+      if constexpr (VALUES) {
+        // a mark in the bucket's high half: it holds two values
+        if ((list[from] ^ e[j]) >> 32) atomicOr(&end[b], 0x10000u);
+      } else {
+        int r = from;
+        for (int i = from; i < last; ++i) r += list[i] > e[j];
+        at[j] = r;
+      }
     }
   __syncthreads();
+  if constexpr (VALUES) {
+#pragma unroll
+    for (int j = 0; j < SF_CAP / SF_THREADS; ++j)
+      if ((int)threadIdx.x + j * SF_THREADS < n) {
+        const int b = bucket(e[j]), last = (int)(end[b] & 0xffffu);
+        if (end[b] >> 16) {
+          int r = b > 0 ? (int)(end[b - 1] & 0xffffu) : 0;
+          const int from = r;
+          for (int i = from; i < last; ++i) r += list[i] > e[j];
+          at[j] = r;
+        }
+      }
+    __syncthreads();
+  }
 #pragma unroll
   for (int j = 0; j < SF_CAP / SF_THREADS; ++j)
     if ((int)threadIdx.x + j * SF_THREADS < n) list[at[j]] = e[j];
@@ -154,7 +181,8 @@ __device__ __forceinline__ void sort_buckets(unsigned long long* list, int n, un
 }
 
 // Sum over the block of each thread's value before this thread (exclusive, in thread order), and the total.
-__device__ __forceinline__ double block_scan(double v, double* red, double* total) {
+// Where only the first `warps` warps have any, theirs are enough.
+__device__ __forceinline__ double block_scan(double v, double* red, double* total, int warps = SF_WARPS) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double s = v;
 #pragma unroll
@@ -165,12 +193,14 @@ __device__ __forceinline__ double block_scan(double v, double* red, double* tota
   __syncthreads();
   if (lane == 31) red[warp] = s;
   __syncthreads();
-  double before = 0.0, all = 0.0;
+  // every warp sums the warps' totals: lane w takes warp w's
+  double p = lane < warps ? red[lane] : 0.0;
 #pragma unroll
-  for (int w = 0; w < SF_WARPS; ++w) {
-    if (w == warp) before = all;
-    all += red[w];
+  for (int o = 1; o < SF_WARPS; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, p, o);
+    if (lane >= o) p += t;
   }
+  const double all = __shfl_sync(0xffffffffu, p, SF_WARPS - 1), before = warp ? __shfl_sync(0xffffffffu, p, warp - 1) : 0.0;
   *total = all;
   return before + (s - v);
 }
@@ -185,12 +215,13 @@ __device__ __forceinline__ float block_scan_f(float v, float* red, float* total)
   __syncthreads();
   if (lane == 31) red[warp] = s;
   __syncthreads();
-  float before = 0.f, all = 0.f;
+  float p = lane < SF_WARPS ? red[lane] : 0.f;
 #pragma unroll
-  for (int w = 0; w < SF_WARPS; ++w) {
-    if (w == warp) before = all;
-    all += red[w];
+  for (int o = 1; o < SF_WARPS; o <<= 1) {
+    const float t = __shfl_up_sync(0xffffffffu, p, o);
+    if (lane >= o) p += t;
   }
+  const float all = __shfl_sync(0xffffffffu, p, SF_WARPS - 1), before = warp ? __shfl_sync(0xffffffffu, p, warp - 1) : 0.f;
   *total = all;
   return before + (s - v);
 }
@@ -205,12 +236,13 @@ __device__ __forceinline__ int block_scan_i(int v, int* red, int* total) {
   __syncthreads();
   if (lane == 31) red[warp] = s;
   __syncthreads();
-  int before = 0, all = 0;
+  int p = lane < SF_WARPS ? red[lane] : 0;
 #pragma unroll
-  for (int w = 0; w < SF_WARPS; ++w) {
-    if (w == warp) before = all;
-    all += red[w];
+  for (int o = 1; o < SF_WARPS; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, p, o);
+    if (lane >= o) p += t;
   }
+  const int all = __shfl_sync(0xffffffffu, p, SF_WARPS - 1), before = warp ? __shfl_sync(0xffffffffu, p, warp - 1) : 0;
   *total = all;
   return before + s - v;
 }
@@ -286,7 +318,9 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   }
   const float itf = a.inv_temp[row] >= 0.f ? fminf(a.inv_temp[row], 1e30f) : 0.f;
   const double it = (double)itf, top = (double)xmax;
-  auto w_of = [&](float x) { return x == xmax ? 1.0 : weight(((double)x - top) * it, sh.tab); };
+  const double top_it = top * it;
+  // the same for every use of a logit: (x - max) * inv_temp in one rounding
+  auto w_of = [&](float x) { return x == xmax ? 1.0 : weight(fma(widen(x), it, -top_it), sh.tab); };
   const bool greedy = a.greedy && a.greedy[row] != 0;
   const float tpf = a.top_p[row];
   const double top_p = (double)fmaxf(tpf, 0.f), min_p = (double)fminf(a.min_p[row], 1.f);
@@ -347,6 +381,39 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   // The list holds, in order, everything that can be kept: what of it is, and the token.
   auto finish = [&](int cnt) {
     const int k = K > 0 ? min(K, cnt) : cnt;
+    if (cnt <= SF_THREADS) {
+      // one thread for each: its place in the sum by index is found by going through them all
+      double* ws = reinterpret_cast<double*>(sh.hist);
+      const unsigned long long e = tid < cnt ? sh.list[tid] : 0ull;
+      const double w = tid < k ? w_of(float_of((unsigned int)(e >> 32))) : 0.0;
+      double sum;
+      const double run = block_scan(w, sh.red, &sum, (cnt + 31) >> 5);
+      const bool kept = w > 0.0 && (!by_mass || run <= top_p * (K > 0 ? sum : total)) && w >= min_p;
+      const int m = max(1, __syncthreads_count(kept));                            // its barrier also ends the use of hist
+      const int index = (int)(0xffffffffu - (unsigned int)e);
+      if (tid < m) ws[tid] = w;
+      if (tid == 0) { sh.cut[0] = 0x7fffffff; sh.cut[1] = -1; }
+      if (tid == m - 1) sh.red2[0] = run + w;
+      __syncthreads();
+      const double all = sh.red2[0], goal = fmax((double)a.u[row], 0.0) * all;
+      if (tid < m) {
+        double q[4] = {0.0, 0.0, 0.0, 0.0};
+        for (int j = 0; j < m; j += 4) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            if (j + h < m && (int)(0xffffffffu - (unsigned int)sh.list[j + h]) <= index) q[h] += ws[j + h];
+        }
+        if ((q[0] + q[1]) + (q[2] + q[3]) > goal) atomicMin(&sh.cut[0], index);
+        atomicMax(&sh.cut[1], index);
+      }
+      __syncthreads();
+      const int tok = sh.cut[0] != 0x7fffffff ? sh.cut[0] : sh.cut[1];
+      if (tid < m && index == tok) {
+        a.out_tok[row] = tok;
+        a.out_logp[row] = (float)log(w / all);
+      }
+      return;
+    }
     double w[4], mine = 0.0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -438,7 +505,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
           if (near) {
             double w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = weight(((double)x[j] - top) * it, sh.tab);
+            for (int j = 0; j < 4; ++j) w[j] = weight(fma(widen(x[j]), it, -top_it), sh.tab);
             s += (w[0] + w[1]) + (w[2] + w[3]);
           } else {
 #pragma unroll
@@ -455,13 +522,18 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       if (lane == 0 && behind) atomicAdd(&sh.hist[SF_BINS - 1], (unsigned int)behind);
       if (by_mass && K == 0) publish_sum(s + (double)far);
     }
+    __syncthreads();
+    {
+      const uint4 v = reinterpret_cast<const uint4*>(sh.hist)[tid];
+      sh.hist16[tid] = make_uint2(v.x | v.y << 16, v.z | v.w << 16);
+    }
     cl.sync();
     if (by_mass && K == 0) { total = all_sum(); buf ^= 1; }
     unsigned int c[4] = {0u, 0u, 0u, 0u};
 #pragma unroll 8
     for (int i = 0; i < nb; ++i) {
-      const uint4 v = reinterpret_cast<const uint4*>(cl.map_shared_rank(sh.hist, i))[tid];
-      c[0] += v.x; c[1] += v.y; c[2] += v.z; c[3] += v.w;
+      const uint2 v = cl.map_shared_rank(sh.hist16, i)[tid];
+      c[0] += v.x & 0xffffu; c[1] += v.x >> 16; c[2] += v.y & 0xffffu; c[3] += v.y >> 16;
     }
     int c_total;
     const int c_before = block_scan_i((int)(c[0] + c[1] + c[2] + c[3]), sh.ired, &c_total);
@@ -548,21 +620,32 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
           if (sure) {
             double w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = t[j] < t_sure ? weight(((double)x[j] - top) * it, sh.tab) : 0.0;
+            for (int j = 0; j < 4; ++j) w[j] = t[j] < t_sure ? weight(fma(widen(x[j]), it, -top_it), sh.tab) : 0.0;
             s += (w[0] + w[1]) + (w[2] + w[3]);
           }
           if (__any_sync(0xffffffffu, some)) {
+            bool take[4];
+            int mine = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const bool take = (to_end || t[j] < t_list) && !(t[j] < t_sure) && x[j] > -INFINITY;
-              const unsigned int who = __ballot_sync(0xffffffffu, take);
-              if (who) {
-                int at = 0;
-                if (lane == 0) at = atomicAdd(&sh.list_n, __popc(who));
-                at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-                if (take && at < SF_CAP) sh.list[at] = ((unsigned long long)key_of(x[j]) << 32) | (0xffffffffu - (unsigned int)(begin + 4 * i + j));
-              }
+              take[j] = (to_end || t[j] < t_list) && !(t[j] < t_sure) && x[j] > -INFINITY;
+              mine += take[j];
             }
+            int at = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int q = __shfl_up_sync(0xffffffffu, at, o);
+              if (lane >= o) at += q;
+            }
+            int base = 0;
+            if (lane == 31 && at) base = atomicAdd(&sh.list_n, at);
+            at += __shfl_sync(0xffffffffu, base, 31) - mine;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (take[j]) {
+                if (at < SF_CAP) sh.list[at] = ((unsigned long long)key_of(x[j]) << 32) | (0xffffffffu - (unsigned int)(begin + 4 * i + j));
+                ++at;
+              }
           }
         }
         if (part) {
@@ -588,14 +671,30 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       int cnt = 0;
       if (me == 0) {
         cnt = min(sh.list_n, SF_CAP);
-        unsigned int at = c_before - (whole ? 0 : before);
-        uint4 e;
-        e.x = at; e.y = at += c[0]; e.z = at += c[1]; e.w = at += c[2];
-        reinterpret_cast<uint4*>(sh.hist)[tid] = e;                               // entries of the list before each bin (of those in it)
-        __syncthreads();
-        if (tid == 0 && b1 > 0 && !whole) sh.hist[b1 - 1] = 0u;
-        __syncthreads();
-        sort_buckets(sh.list, cnt, sh.hist, [&](unsigned long long q) { return (int)fminf((xmax - float_of((unsigned int)(q >> 32))) * scale, (float)(SF_BINS - 1)); });
+        if (whole) {
+          unsigned int at = c_before;
+          uint4 e;
+          e.x = at; e.y = at += c[0]; e.z = at += c[1]; e.w = at += c[2];
+          reinterpret_cast<uint4*>(sh.hist)[tid] = e;                             // entries before each bin
+          __syncthreads();
+          sort_buckets(sh.list, cnt, sh.hist, [&](unsigned long long q) { return (int)fminf((xmax - float_of((unsigned int)(q >> 32))) * scale, (float)(SF_BINS - 1)); });
+        } else {
+          // the undecided bins hold a sixty-fourth of a nat each: cut again, finely enough that most buckets hold one value
+          const float fine = (float)(SF_BINS - 1) / (float)(b2 + 1 - b1);
+          auto bucket = [&](unsigned long long q) {
+            return (int)fmaxf(fminf(((xmax - float_of((unsigned int)(q >> 32))) * scale - t_sure) * fine, (float)(SF_BINS - 1)), 0.f);
+          };
+          for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
+          __syncthreads();
+          for (int i = tid; i < cnt; i += SF_THREADS) atomicAdd(&sh.hist[bucket(sh.list[i])], 1u);
+          __syncthreads();
+          const uint4 q = reinterpret_cast<const uint4*>(sh.hist)[tid];
+          int all_i;
+          const unsigned int at = block_scan_i((int)(q.x + q.y + q.z + q.w), sh.ired, &all_i);
+          reinterpret_cast<uint4*>(sh.hist)[tid] = make_uint4(at, at + q.x, at + q.x + q.y, at + q.x + q.y + q.z);
+          __syncthreads();
+          sort_buckets<true>(sh.list, cnt, sh.hist, bucket);
+        }
       }
       if (whole) {
         finish(cnt);
