@@ -29,6 +29,7 @@ constexpr int SF_CAP = 2048;           // entries of the list
 constexpr int SF_SEG = 256;            // logits of a piece of a block's share that has a sum of its own
 constexpr int SF_SEGS = 200;           // at most
 constexpr float SF_FAR = 16.6f;        // nats below the maximum from where single precision will do for a total (2^-24 of the maximum)
+constexpr int SF_GUESS = 256;           // tokens of a nucleus that is tried without a histogram of the row
 constexpr int SF_MAX_CLUSTER = 8;
 constexpr float SF_PER_NAT = 64.f;
 
@@ -48,6 +49,7 @@ struct SampleArgs {
 struct SampleShared {
   unsigned long long list[SF_CAP];
   unsigned int hist[SF_BINS];
+  float peak[SF_THREADS];              // the largest logit of each thread's
   uint2 hist16[SF_BINS / 4];           // the same in 16 bits, for the other blocks (a share is below 65536)
   double tab[32];                      // 2^(j/32): the entries of a half warp fall on banks of their own
   double seg_sum[SF_SEGS];
@@ -77,7 +79,7 @@ __device__ __forceinline__ double weight(double d, const double* tab) {
   const double w = p * tab[k & 31];
   // e^-700 and less (the high word of a negative number rises as it falls; minus infinity and NaN are above them all): zero
   const bool gone = (unsigned int)__double2hiint(d) > 0xc085e000u;
-  return __hiloint2double(gone ? 0 : __double2hiint(w) + ((k >> 5) << 20), gone ? 0 : __double2loint(w));
+  return __hiloint2double(gone ? 0 : __double2hiint(w) + ((k >> 5) << 20), __double2loint(w));      // (below 1e-307 where gone)
 }
 // float -> double by its bits, off the 64-bit pipe. Denormal numbers come out as ones of their order; infinities as +-2^128.
 __device__ __forceinline__ double widen(float x) {
@@ -267,7 +269,6 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   const int row = blockIdx.x / nb, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_trigger();
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");          // met below: every block runs before its memory is written from outside
   const int begin = min(me * a.share, a.V), n = min(a.share, a.V - begin);       // this block's logits
   int buf = 0;                                                                   // set of the published values in use
   // ---- the row into shared memory, its maximum
@@ -293,29 +294,30 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
   if (tid < 32) sh.tab[tid] = a.tab[tid];
   if (tid == 0) sh.list_n = 0;
-  mx = warp_max(mx);
-  if (lane == 0) sh.fred[0][warp] = mx;
-  __syncthreads();
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-  if (tid < nb) {
-    float m = sh.fred[0][0];
-#pragma unroll
-    for (int w = 1; w < SF_WARPS; ++w) m = fmaxf(m, sh.fred[0][w]);
-    cl.map_shared_rank(&sh, tid)->pub_hi[buf][me] = m;
-  }
+  sh.peak[tid] = mx;
   cl.sync();
-  float xmax = -INFINITY;
-  for (int i = 0; i < nb; ++i) xmax = fmaxf(xmax, sh.pub_hi[buf][i]);
-  buf ^= 1;
+  float peaks[SF_MAX_CLUSTER], xmax = -INFINITY;                                 // every block looks at all threads' largest
+#pragma unroll
+  for (int i = 0; i < SF_MAX_CLUSTER; ++i) {
+    peaks[i] = i < nb ? cl.map_shared_rank(sh.peak, i)[tid] : -INFINITY;
+    xmax = fmaxf(xmax, peaks[i]);
+  }
+  xmax = warp_max(xmax);
+  if (lane == 0) sh.fred[0][warp] = xmax;
+  __syncthreads();
+  xmax = warp_max(sh.fred[0][lane % SF_WARPS]);
   if (xmax == -INFINITY) {                                                       // nothing has any weight
     if (me == 0 && tid == 0) { a.out_tok[row] = -1; a.out_logp[row] = -INFINITY; }
+    cl.sync();                                                                   // the others may still be reading this block's peaks
     return;
   }
   if (xmax == INFINITY) {                                                        // only infinite logits have weight, all the same
-    for (int i = tid; i < n; i += SF_THREADS) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+    for (int i = tid; i < a.share; i += SF_THREADS) xs[i] = xs[i] == INFINITY ? 0.f : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < SF_MAX_CLUSTER; ++i) peaks[i] = peaks[i] == INFINITY ? 0.f : -INFINITY;
     xmax = 0.f;
-    __syncthreads();
   }
+  __syncthreads();
   const float itf = a.inv_temp[row] >= 0.f ? fminf(a.inv_temp[row], 1e30f) : 0.f;
   const double it = (double)itf, top = (double)xmax;
   const double top_it = top * it;
@@ -434,6 +436,36 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     int m;
     block_scan_i(kept, sh.ired, &m);
     if (m == 0) m = 1;
+    // a long list is in order by value only: of the entries equal to the last kept one, those with the lowest indices go first
+    const unsigned int edge = (unsigned int)(sh.list[m - 1] >> 32);
+    if (m < cnt && (unsigned int)(sh.list[m] >> 32) == edge) {
+      int above = 0, same = 0;
+      for (int i = tid; i < cnt; i += SF_THREADS) {
+        const unsigned int v = (unsigned int)(sh.list[i] >> 32);
+        above += v > edge;
+        same += v == edge;
+      }
+      int from, size;
+      block_scan_i(above, sh.ired, &from);
+      block_scan_i(same, sh.ired, &size);
+      unsigned long long e[SF_CAP / SF_THREADS];
+      int at[SF_CAP / SF_THREADS];
+#pragma unroll
+      for (int j = 0; j < SF_CAP / SF_THREADS; ++j) {
+        const int i = tid + j * SF_THREADS;
+        at[j] = -1;
+        if (i >= from && i < from + size) {
+          e[j] = sh.list[i];
+          at[j] = from;
+          for (int q = from; q < from + size; ++q) at[j] += sh.list[q] > e[j];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < SF_CAP / SF_THREADS; ++j)
+        if (at[j] >= 0) sh.list[at[j]] = e[j];
+    }
+    __syncthreads();
     // the kept ones by index: the key's low half, the index's complement, to the front
     for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
     __syncthreads();
@@ -482,14 +514,185 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   const int n4 = a.share / 4, segs = (a.share + SF_SEG - 1) / SF_SEG;
   const float4* xs4 = reinterpret_cast<const float4*>(xs);
   bool decided = !(K > 0 || by_mass || by_min);         // thr and ties are known
-  bool summed = false;                                   // seg_sum has the weights of what is before t_sure
-  float t_sure = 0.f;                                    // in bins below the maximum: what is before is kept, whatever thr is
-  const float scale = itf * SF_PER_NAT;
-  if (!decided) {
-    {
-      double s = 0.0;
+  bool summed = false;                                   // s_own has this block's weights before t_sure
+  double s_own = 0.0;
+  float t_sure = -INFINITY;                              // a depth: what is before is kept, whatever thr is
+  const float scale = itf * SF_PER_NAT, top_t = xmax * scale;
+  // how far a logit is below the largest, in bins of 1/64 nat: one rounding, so it falls as the logit rises; off by 1e-3 bins at most
+  // as long as `plain` holds (within 300 nats of zero: any sane row), else the general way below takes the row
+  auto depth = [&](float x) { return fmaf(x, -scale, top_t); };
+  const bool plain = itf >= 1e-6f && fabsf(top_t) < 300.f * SF_PER_NAT;
+  bool have_total = false;
+  // ---- a list guessed from the peaks: the k-th largest of the threads' largest logits bounds the k-th largest logit, so its bin and those
+  // before hold k tokens at least and usually few more; for top-p it is a guess (SF_GUESS tokens), which the sums confirm or not
+  if (plain && !decided && K <= nb * (SF_THREADS / 4)) {
+    const int want = K > 0 ? K : SF_GUESS;
+    float t_list = INFINITY;
+    bool from_min = false;                               // what is not listed is dropped by min-p
+    bool guess = true;
+    if (K > 0 || by_mass) {
+#pragma unroll
+      for (int i = 0; i < SF_MAX_CLUSTER; ++i) {
+        const float t = depth(peaks[i]);
+        if (t < (float)(SF_BINS - 1)) atomicAdd(&sh.hist[__float2uint_rz(t)], 1u);
+      }
+      if (tid == 0) sh.cut[0] = SF_BINS;
+      __syncthreads();
+      const uint4 c = reinterpret_cast<const uint4*>(sh.hist)[tid];
+      int all_i;
+      int at = block_scan_i((int)(c.x + c.y + c.z + c.w), sh.ired, &all_i);
+      const unsigned int cc[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (at < want && at + (int)cc[j] >= want) sh.cut[0] = 4 * tid + j;
+        at += (int)cc[j];
+      }
+      if (by_mass && K == 0) {
+        // the peaks' own weights, those in front against all: a share below top_p already says that the nucleus is longer
+        float e = fast_exp2(tid * (-4.f * 1.4426950408889634f / SF_PER_NAT)), m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { m += (float)cc[j] * e; e *= 0.98449643700540842f; }
+        float m_all;
+        const float m_before = block_scan_f(m, sh.fred[1], &m_all);
+        if (sh.cut[0] < SF_BINS && sh.cut[0] >> 2 == tid) sh.fred[3][0] = m_before + m;
+        __syncthreads();
+        guess = sh.cut[0] >= SF_BINS || sh.fred[3][0] > (float)top_p * m_all;
+      }
+      reinterpret_cast<uint4*>(sh.hist)[tid] = make_uint4(0u, 0u, 0u, 0u);
+      __syncthreads();
+      if (sh.cut[0] < SF_BINS) t_list = (float)(sh.cut[0] + 1);                   // the last bin is not counted above
+    }
+    if (by_min && !(K > 0 && by_mass)) {
+      const float t = (float)(-log(min_p)) * SF_PER_NAT * 1.0001f + 1.f;          // ln(1 / min_p), and what rounding does to it
+      if (t <= t_list) { t_list = t; from_min = guess = true; }
+    }
+    if (guess) {
+      const bool to_end = t_list == INFINITY, sums = by_mass && K == 0;
+      double s = 0.0, s_head = 0.0;
       float far = 0.f;
-      int behind = 0;
+      int listed = 0;                                      // lane 31: entries of this warp
+#pragma unroll 2
+      for (int i0 = 0; i0 < n4; i0 += SF_THREADS) {
+        const int i = i0 + tid;
+        const float4 v = i < n4 ? xs4[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        float t[4];
+        bool some = to_end, near = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          t[j] = depth(x[j]);
+          some |= t[j] < t_list;
+          near |= t[j] < SF_FAR * SF_PER_NAT;
+        }
+        if (sums) {
+          if (near) {
+            double w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = weight(fma(widen(x[j]), it, -top_it), sh.tab);
+            s += (w[0] + w[1]) + (w[2] + w[3]);
+            if (some) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s_head += to_end || t[j] < t_list ? w[j] : 0.0;
+            }
+          } else {
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              f[j] = fast_exp2(t[j] * (-1.4426950408889634f / SF_PER_NAT));
+              far += f[j];
+            }
+            if (some) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s_head += to_end || t[j] < t_list ? (double)f[j] : 0.0;
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, some)) {
+          int mine = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mine += (to_end || t[j] < t_list) && x[j] > -INFINITY;
+          int at = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int q = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += q;
+          }
+          int base = 0;
+          if (lane == 31 && at) base = atomicAdd(&sh.list_n, at);
+          listed += at;
+          at += __shfl_sync(0xffffffffu, base, 31) - mine;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((to_end || t[j] < t_list) && x[j] > -INFINITY) {
+              if (at < SF_CAP) sh.list[at] = ((unsigned long long)key_of(x[j]) << 32) | (0xffffffffu - (unsigned int)(begin + 4 * i + j));
+              ++at;
+            }
+        }
+      }
+      if (lane == 31) sh.seg_tie[warp] = listed;
+      __syncthreads();
+      if (me != 0) {                                                                // the first block's list takes them all
+        SampleShared* head = cl.map_shared_rank(&sh, 0);
+        const int k = sh.list_n;
+        if (tid == 0 && k) sh.ired[0] = atomicAdd(&head->list_n, k);
+        __syncthreads();
+        const int at = sh.ired[0];
+        for (int i = tid; i < k && at + i < SF_CAP; i += SF_THREADS) head->list[at + i] = sh.list[i];
+      }
+      if (sums) {
+        s = warp_sum_d(s + (double)far);
+        s_head = warp_sum_d(s_head);
+        if (lane == 0) { sh.red[warp] = s; sh.red2[warp] = s_head; }
+      }
+      __syncthreads();
+      if (tid < nb) {
+        double q = 0.0, q2 = 0.0;
+        int k = 0;
+#pragma unroll
+        for (int w = 0; w < SF_WARPS; ++w) {
+          if (sums) { q += sh.red[w]; q2 += sh.red2[w]; }
+          k += sh.seg_tie[w];
+        }
+        SampleShared* o = cl.map_shared_rank(&sh, tid);
+        o->pub_sum[buf][me] = q;
+        o->pub_sum2[buf][me] = q2;
+        o->pub_int[buf][me] = k;
+      }
+      cl.sync();
+      double in_list = 0.0;
+      int cnt = 0;
+      for (int i = 0; i < nb; ++i) { in_list += sh.pub_sum2[buf][i]; cnt += sh.pub_int[buf][i]; }
+      if (sums) total = all_sum();
+      have_total = sums;
+      buf ^= 1;
+      if (cnt <= SF_CAP && (!sums || to_end || from_min || in_list > top_p * total)) {
+        if (me != 0) return;
+        const float fine = to_end ? 1.f : (float)(SF_BINS - 1) / t_list;
+        auto bucket = [&](unsigned long long q) { return (int)fmaxf(fminf(depth(float_of((unsigned int)(q >> 32))) * fine, (float)(SF_BINS - 1)), 0.f); };
+        for (int i = tid; i < cnt; i += SF_THREADS) atomicAdd(&sh.hist[bucket(sh.list[i])], 1u);
+        __syncthreads();
+        const uint4 q = reinterpret_cast<const uint4*>(sh.hist)[tid];
+        int all_i;
+        const unsigned int at = block_scan_i((int)(q.x + q.y + q.z + q.w), sh.ired, &all_i);
+        reinterpret_cast<uint4*>(sh.hist)[tid] = make_uint4(at, at + q.x, at + q.x + q.y, at + q.x + q.y + q.z);
+        __syncthreads();
+        if (cnt <= SF_THREADS) sort_buckets(sh.list, cnt, sh.hist, bucket);
+        else sort_buckets<true>(sh.list, cnt, sh.hist, bucket);
+        finish(cnt);
+        return;
+      }
+    }
+    if (tid == 0) sh.list_n = 0;
+    decided = K == 0 && !by_mass;                        // min-p alone: every token is looked at anyway
+    __syncthreads();
+  }
+  if (plain && !decided) {
+    {
+      // logits without weight fall into the last bin, which is open below. The shared-memory atomics bound this loop; the exact sums that
+      // top-p needs fit between them.
+      const bool sums = by_mass && K == 0 && !have_total;
+      double q = 0.0;
+      float far = 0.f;
 #pragma unroll 2
       for (int i = tid; i < n4; i += SF_THREADS) {
         const float4 v = xs4[i];
@@ -498,29 +701,23 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
         bool near = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          t[j] = (xmax - x[j]) * scale;
+          t[j] = depth(x[j]);
           near |= t[j] < SF_FAR * SF_PER_NAT;
+          atomicAdd(&sh.hist[__float2uint_rz(fminf(t[j], (float)(SF_BINS - 1)))], 1u);
         }
-        if (by_mass && K == 0) {
+        if (sums) {
           if (near) {
             double w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = weight(fma(widen(x[j]), it, -top_it), sh.tab);
-            s += (w[0] + w[1]) + (w[2] + w[3]);
+            q += (w[0] + w[1]) + (w[2] + w[3]);
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) far += fast_exp2(t[j] * (-1.4426950408889634f / SF_PER_NAT));
           }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (t[j] < (float)(SF_BINS - 1)) atomicAdd(&sh.hist[(int)t[j]], 1u);
-          else if (x[j] > -INFINITY) ++behind;
-        }
       }
-      behind = warp_sum_i(behind);
-      if (lane == 0 && behind) atomicAdd(&sh.hist[SF_BINS - 1], (unsigned int)behind);
-      if (by_mass && K == 0) publish_sum(s + (double)far);
+      if (sums) publish_sum(q + (double)far);
     }
     __syncthreads();
     {
@@ -528,7 +725,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       sh.hist16[tid] = make_uint2(v.x | v.y << 16, v.z | v.w << 16);
     }
     cl.sync();
-    if (by_mass && K == 0) { total = all_sum(); buf ^= 1; }
+    if (by_mass && K == 0 && !have_total) { total = all_sum(); buf ^= 1; }
     unsigned int c[4] = {0u, 0u, 0u, 0u};
 #pragma unroll 8
     for (int i = 0; i < nb; ++i) {
@@ -538,99 +735,91 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     int c_total;
     const int c_before = block_scan_i((int)(c[0] + c[1] + c[2] + c[3]), sh.ired, &c_total);
     K = min(K, c_total);                                                          // no more tokens than that have any weight
-    if (tid == 0) { sh.cut[0] = SF_BINS; sh.cut[1] = SF_BINS; sh.cut[2] = c_total; sh.cut[3] = 0; }
-    __syncthreads();
-    if (K > 0) {
-      int at = c_before;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (at < K && at + (int)c[j] >= K) { sh.cut[0] = 0; sh.cut[1] = 4 * tid + j; sh.cut[2] = at + (int)c[j]; sh.cut[3] = 0; }
-        at += (int)c[j];
-      }
-    } else if (by_mass && total > 0.0) {
-      // a bin's weights lie between those of its edges, exp(-b / 64) and exp(-(b + 1) / 64), but for the open last one: from those, bounds
-      // on what is before and behind a bin's end. Single precision, and the rounding of x to its bin, stay well within `slack`.
-      const float f = 0.98449643700540842f, slack = 4e-5f;                        // exp(-1 / 64)
-      const float w0 = fast_exp2(tid * (-4.f * 1.4426950408889634f / SF_PER_NAT));
-      float lo[4], m = 0.f, e = w0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        e *= f;
-        lo[j] = 4 * tid + j < SF_BINS - 1 ? (float)c[j] * e : 0.f;
-        m += lo[j];
-      }
-      float m_all;
-      float m_cum = block_scan_f(m, sh.fred[0], &m_all);
-      if (tid == SF_THREADS - 1) sh.fred[1][0] = (float)c[3] * e / f;
+    do {
+      if (tid == 0) { sh.cut[0] = SF_BINS; sh.cut[1] = SF_BINS; sh.cut[2] = c_total; sh.cut[3] = 0; }
       __syncthreads();
-      const float last_hi = sh.fred[1][0], want = (float)(top_p * total), rest = (float)(total - top_p * total);
-      int at = c_before, b1 = SF_BINS, b2 = SF_BINS, c1 = 0, c2 = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m_cum += lo[j];
-        const bool end = 4 * tid + j == SF_BINS - 1;
-        const float behind = fmaxf(m_all - m_cum, 0.f), fuzz = slack * m_all;     // the difference of two sums is off by a part of them
-        const bool maybe = c[j] && (end || (m_cum / f * (1.f + slack) > want && (behind - fuzz) * (1.f - slack) < rest));
-        const bool sure = c[j] && (end || m_cum * (1.f - slack) > want || ((behind + fuzz) / f + last_hi) * (1.f + slack) < rest);
-        if (maybe && b1 == SF_BINS) { b1 = 4 * tid + j; c1 = at; }
-        at += (int)c[j];
-        if (sure && b2 == SF_BINS) { b2 = 4 * tid + j; c2 = at; }
-      }
-      if (b1 < SF_BINS) atomicMin(&sh.cut[0], b1);
-      if (b2 < SF_BINS) atomicMin(&sh.cut[1], b2);
-      __syncthreads();
-      if (b1 < SF_BINS && sh.cut[0] == b1) sh.cut[3] = c1;
-      if (b2 < SF_BINS && sh.cut[1] == b2) sh.cut[2] = c2;
-    } else if (by_min) {
-      // ln(1 / min_p) below the maximum, a bin further for what rounding does to the edges
-      const double t = -log(min_p) * (double)SF_PER_NAT + 1.0;
-      const int b2 = t < (double)(SF_BINS - 1) ? (int)t : SF_BINS - 1;
-      if (tid == b2 >> 2) {
+      if (K > 0) {
         int at = c_before;
-        for (int j = 0; j <= (b2 & 3); ++j) at += (int)c[j];
-        sh.cut[0] = 0; sh.cut[1] = b2; sh.cut[2] = at; sh.cut[3] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (at < K && at + (int)c[j] >= K) { sh.cut[0] = 0; sh.cut[1] = 4 * tid + j; sh.cut[2] = at + (int)c[j]; sh.cut[3] = 0; }
+          at += (int)c[j];
+        }
+      } else if (by_mass) {
+        const float f = 0.98449643700540842f, slack = 4e-5f;                      // exp(-1 / 64)
+        const float w0 = fast_exp2(tid * (-4.f * 1.4426950408889634f / SF_PER_NAT));
+        float part[4], m = 0.f, e = w0;                                           // the bins' masses from below
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          part[j] = 4 * tid + j < SF_BINS - 1 ? (float)c[j] * e * f : 0.f;
+          m += part[j];
+          e *= f;
+        }
+        float m_all;
+        float m_cum = block_scan_f(m, sh.fred[0], &m_all);
+        if (tid == SF_THREADS - 1) sh.fred[1][0] = (float)c[3] * e / f;           // the open last bin, from above
+        __syncthreads();
+        const float last_hi = sh.fred[1][0];
+        const float want = (float)(top_p * total), rest = (float)(total - top_p * total);
+        int at = c_before, b1 = SF_BINS, b2 = SF_BINS, c1 = 0, c2 = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m_cum += part[j];
+          const bool end = 4 * tid + j == SF_BINS - 1;
+          // a bin's weights lie between those of its edges, but for the last one: from those, bounds on what is before and behind a
+          // bin's end. Single precision, and the rounding of x to its bin, stay well within `slack`.
+          const float behind = fmaxf(m_all - m_cum, 0.f), fuzz = slack * m_all;                  // the difference of two sums is off by a part of them
+          const bool maybe = m_cum / f * (1.f + slack) > want && (behind - fuzz) * (1.f - slack) < rest;
+          const bool sure = m_cum * (1.f - slack) > want || ((behind + fuzz) / f + last_hi) * (1.f + slack) < rest;
+          if (c[j] && (maybe || end) && b1 == SF_BINS) { b1 = 4 * tid + j; c1 = at; }
+          at += (int)c[j];
+          if (c[j] && (sure || end) && b2 == SF_BINS) { b2 = 4 * tid + j; c2 = at; }
+        }
+        if (b1 < SF_BINS) atomicMin(&sh.cut[0], b1);
+        if (b2 < SF_BINS) atomicMin(&sh.cut[1], b2);
+        __syncthreads();
+        if (b1 < SF_BINS && sh.cut[0] == b1) sh.cut[3] = c1;
+        if (b2 < SF_BINS && sh.cut[1] == b2) sh.cut[2] = c2;
       }
-    }
-    __syncthreads();
-    int b1 = sh.cut[0], b2 = sh.cut[1], before = sh.cut[3];
-    const int upto = sh.cut[2];
-    if (b2 >= SF_BINS) b2 = SF_BINS - 1;
-    if (b1 > b2) b1 = before = 0;
-    const bool whole = upto <= SF_CAP, part = !whole && K == 0 && by_mass && upto - before <= SF_CAP;
-    if (whole || part) {
+      __syncthreads();
+      int b1 = sh.cut[0], b2 = sh.cut[1], before = sh.cut[3];
+      const int upto = sh.cut[2];
+      if (b2 >= SF_BINS) b2 = SF_BINS - 1;
+      if (b1 > b2) b1 = before = 0;
+      const bool whole = upto <= SF_CAP, part = !whole && K == 0 && upto - before <= SF_CAP;
+      if (!whole && !part) break;
       const bool to_end = b2 == SF_BINS - 1;
       const float t_list = (float)(b2 + 1);
-      t_sure = whole ? 0.f : (float)b1;
+      t_sure = part && b1 > 0 ? (float)b1 : -INFINITY;                            // (the largest logit may be a rounding before zero)
+      const float t_from = whole ? 0.f : (float)b1;
       SampleShared* head = cl.map_shared_rank(&sh, 0);
-      for (int g = warp; g < segs; g += SF_WARPS) {
-        double s = 0.0;
-#pragma unroll
-        for (int h = 0; h < SF_SEG / 128; ++h) {
-          const int i = g * (SF_SEG / 4) + h * 32 + lane;
+      double s = 0.0;
+#pragma unroll 2
+      for (int i0 = 0; i0 < n4; i0 += SF_THREADS) {
+        {
+          const int i = i0 + tid;
           const float4 v = i < n4 ? xs4[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
           const float x[4] = {v.x, v.y, v.z, v.w};
           float t[4];
-          bool some = to_end, sure = false;
+          bool some = false, sure = false;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            t[j] = (xmax - x[j]) * scale;
-            some |= t[j] < t_list;
+            t[j] = depth(x[j]);
+            some |= (to_end || t[j] < t_list) && !(t[j] < t_sure);
             sure |= t[j] < t_sure;
           }
           if (sure) {
             double w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = t[j] < t_sure ? weight(fma(widen(x[j]), it, -top_it), sh.tab) : 0.0;
+            for (int j = 0; j < 4; ++j) w[j] = weight(fma(widen(x[j]), it, -top_it), sh.tab);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = t[j] < t_sure ? w[j] : 0.0;
             s += (w[0] + w[1]) + (w[2] + w[3]);
           }
           if (__any_sync(0xffffffffu, some)) {
-            bool take[4];
             int mine = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              take[j] = (to_end || t[j] < t_list) && !(t[j] < t_sure) && x[j] > -INFINITY;
-              mine += take[j];
-            }
+            for (int j = 0; j < 4; ++j) mine += (to_end || t[j] < t_list) && !(t[j] < t_sure) && x[j] > -INFINITY;
             int at = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -642,66 +831,51 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
             at += __shfl_sync(0xffffffffu, base, 31) - mine;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (take[j]) {
+              if ((to_end || t[j] < t_list) && !(t[j] < t_sure) && x[j] > -INFINITY) {
                 if (at < SF_CAP) sh.list[at] = ((unsigned long long)key_of(x[j]) << 32) | (0xffffffffu - (unsigned int)(begin + 4 * i + j));
                 ++at;
               }
           }
         }
-        if (part) {
-          s = warp_sum_d(s);
-          if (lane == 0) sh.seg_sum[g] = s;
-        }
       }
       __syncthreads();
-      if (me != 0) {                                                              // the first block's list takes them all
+      if (me != 0) {                                                   // the first block's list takes them all
         const int k = sh.list_n;
         if (tid == 0 && k) sh.ired[0] = atomicAdd(&head->list_n, k);
         __syncthreads();
         const int at = sh.ired[0];
         for (int i = tid; i < k && at + i < SF_CAP; i += SF_THREADS) head->list[at + i] = sh.list[i];
       }
-      if (part) {
-        double s = 0.0;
-        for (int g = tid; g < segs; g += SF_THREADS) s += sh.seg_sum[g];
-        publish_sum(s);
-      }
+      publish_sum(s);
       cl.sync();
+      const double s_above = all_sum();
+      s_own = sh.pub_sum[buf][me];
+      buf ^= 1;
       if (whole && me != 0) return;
-      int cnt = 0;
+      const int cnt = me == 0 ? min(sh.list_n, SF_CAP) : 0;
       if (me == 0) {
-        cnt = min(sh.list_n, SF_CAP);
-        if (whole) {
-          unsigned int at = c_before;
-          uint4 e;
-          e.x = at; e.y = at += c[0]; e.z = at += c[1]; e.w = at += c[2];
-          reinterpret_cast<uint4*>(sh.hist)[tid] = e;                             // entries before each bin
-          __syncthreads();
-          sort_buckets(sh.list, cnt, sh.hist, [&](unsigned long long q) { return (int)fminf((xmax - float_of((unsigned int)(q >> 32))) * scale, (float)(SF_BINS - 1)); });
-        } else {
-          // the undecided bins hold a sixty-fourth of a nat each: cut again, finely enough that most buckets hold one value
-          const float fine = (float)(SF_BINS - 1) / (float)(b2 + 1 - b1);
-          auto bucket = [&](unsigned long long q) {
-            return (int)fmaxf(fminf(((xmax - float_of((unsigned int)(q >> 32))) * scale - t_sure) * fine, (float)(SF_BINS - 1)), 0.f);
-          };
-          for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
-          __syncthreads();
-          for (int i = tid; i < cnt; i += SF_THREADS) atomicAdd(&sh.hist[bucket(sh.list[i])], 1u);
-          __syncthreads();
-          const uint4 q = reinterpret_cast<const uint4*>(sh.hist)[tid];
-          int all_i;
-          const unsigned int at = block_scan_i((int)(q.x + q.y + q.z + q.w), sh.ired, &all_i);
-          reinterpret_cast<uint4*>(sh.hist)[tid] = make_uint4(at, at + q.x, at + q.x + q.y, at + q.x + q.y + q.z);
-          __syncthreads();
-          sort_buckets<true>(sh.list, cnt, sh.hist, bucket);
-        }
+        // order: by bins of the list's own range, finely enough that most hold one value. Of equal values the lowest index comes first only
+        // where the list is all there is; for the last kept value and its number the order among them does not matter.
+        const float fine = (float)(SF_BINS - 1) / (t_list - t_from);
+        auto bucket = [&](unsigned long long q) {
+          return (int)fmaxf(fminf((depth(float_of((unsigned int)(q >> 32))) - t_from) * fine, (float)(SF_BINS - 1)), 0.f);
+        };
+        for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
+        __syncthreads();
+        for (int i = tid; i < cnt; i += SF_THREADS) atomicAdd(&sh.hist[bucket(sh.list[i])], 1u);
+        __syncthreads();
+        const uint4 q = reinterpret_cast<const uint4*>(sh.hist)[tid];
+        int all_i;
+        const unsigned int at = block_scan_i((int)(q.x + q.y + q.z + q.w), sh.ired, &all_i);
+        reinterpret_cast<uint4*>(sh.hist)[tid] = make_uint4(at, at + q.x, at + q.x + q.y, at + q.x + q.y + q.z);
+        __syncthreads();
+        if (whole && cnt <= SF_THREADS) sort_buckets(sh.list, cnt, sh.hist, bucket);
+        else sort_buckets<true>(sh.list, cnt, sh.hist, bucket);
       }
       if (whole) {
         finish(cnt);
         return;
       }
-      const double s_above = all_sum();
-      buf ^= 1;
       if (me == 0) {
         double w[4], mine = 0.0;
 #pragma unroll
@@ -727,6 +901,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
           if (4 * tid + j < m && (unsigned int)(sh.list[4 * tid + j] >> 32) == last) ++same;
         int eq;
         block_scan_i(same, sh.ired, &eq);
+        __syncthreads();
         if (tid < nb) {
           SampleShared* o = cl.map_shared_rank(&sh, tid);
           // nothing of the list kept (the border at its very start): what is above it, up to the lowest value that is
@@ -739,9 +914,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       ties = sh.ties;
       decided = true;
       summed = !by_min;                                                           // min-p may take some of those away
-    } else if (K == 0 && !by_mass) {
-      decided = true;                                                             // min-p alone: every token is looked at anyway
-    }
+    } while (false);
     if (!decided) {
       cl.sync();                                                                  // every block has read the histograms
       for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
@@ -1029,55 +1202,49 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     __syncthreads();
   }
 
-  // ---- kept weights summed by index: pieces of the block's share, blocks, row
-  for (int g = warp; g < segs; g += SF_WARPS) {
+  // ---- kept weights by index: sums of the blocks, and in the block that has the token sums of pieces of its share
+  {
     double s = 0.0;
     int eq = 0;
-    bool some = false;
-#pragma unroll
-    for (int h = 0; h < SF_SEG / 128; ++h) {
-      const int i = g * (SF_SEG / 4) + h * 32 + lane;
-      const float4 v = i < n4 ? xs4[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll 2
+    for (int i = tid; i < n4; i += SF_THREADS) {
+      const float4 v = xs4[i];
       const float x[4] = {v.x, v.y, v.z, v.w};
-      double w[4];
+      bool in[4], any = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const bool sure = (xmax - x[j]) * scale < t_sure;
-        const bool new_one = summed ? x[j] > thr && !sure : x[j] > thr || sure;
-        w[j] = 0.0;
-        if (new_one) {
-          w[j] = w_of(x[j]);
-          some = true;
-        }
-        if (w[j] < min_p) w[j] = 0.0;
-        if (x[j] == thr && x[j] != -INFINITY) { ++eq; some = true; }
+        const bool sure = depth(x[j]) < t_sure;
+        in[j] = summed ? x[j] > thr && !sure : x[j] > thr || sure;                // those before t_sure are in the sum already
+        any |= in[j];
+        eq += x[j] == thr && x[j] != -INFINITY;
       }
-      s += (w[0] + w[1]) + (w[2] + w[3]);
+      if (any) {
+        double w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[j] = weight(fma(widen(x[j]), it, -top_it), sh.tab);
+          if (!in[j] || w[j] < min_p) w[j] = 0.0;
+        }
+        s += (w[0] + w[1]) + (w[2] + w[3]);
+      }
     }
-    if (!summed || __any_sync(0xffffffffu, some)) {
-      s = warp_sum_d(s);
-      eq = warp_sum_i(eq);
-    }
-    if (lane == 0) {
-      sh.seg_sum[g] = summed ? sh.seg_sum[g] + s : s;
-      sh.seg_tie[g] = eq;
-    }
-  }
-  __syncthreads();
-  double w_tie = thr == -INFINITY ? 0.0 : w_of(thr);
-  if (w_tie < min_p) w_tie = 0.0;
-  if (warp == 0) {
-    double s = 0.0;
-    int eq = 0;
-    for (int g = lane; g < segs; g += 32) { s += sh.seg_sum[g]; eq += sh.seg_tie[g]; }
     s = warp_sum_d(s);
     eq = warp_sum_i(eq);
-    if (lane < nb) {
-      SampleShared* t = cl.map_shared_rank(&sh, lane);
+    __syncthreads();
+    if (lane == 0) { sh.red[warp] = s; sh.ired[warp] = eq; }
+    __syncthreads();
+    if (tid < nb) {
+      s = summed ? s_own : 0.0;
+      eq = 0;
+#pragma unroll
+      for (int w = 0; w < SF_WARPS; ++w) { s += sh.red[w]; eq += sh.ired[w]; }
+      SampleShared* t = cl.map_shared_rank(&sh, tid);
       t->pub_sum[buf][me] = s;
       t->pub_int[buf][me] = eq;
     }
   }
+  double w_tie = thr == -INFINITY || thr == INFINITY ? 0.0 : w_of(thr);
+  if (w_tie < min_p) w_tie = 0.0;
   cl.sync();
   double sum = 0.0, my_begin = 0.0, my_sum = 0.0;
   int ties_left = ties, my_ties = 0, last = 0;
@@ -1092,7 +1259,30 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   const double goal = fmax((double)a.u[row], 0.0) * sum;
   // the first block whose end passes the goal (the last one with any weight, should rounding leave none)
   const bool mine = my_sum > 0.0 && my_begin <= goal && (my_begin + my_sum > goal || me == last);
-  if (!mine || warp != 0) return;
+  if (!mine) return;
+  for (int g = warp; g < segs; g += SF_WARPS) {
+    double s = 0.0;
+    int eq = 0;
+#pragma unroll
+    for (int h = 0; h < SF_SEG / 128; ++h) {
+      const int i = g * (SF_SEG / 4) + h * 32 + lane;
+      const float4 v = i < n4 ? xs4[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      double w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = weight(fma(widen(x[j]), it, -top_it), sh.tab);
+        if (!(x[j] > thr || depth(x[j]) < t_sure) || w[j] < min_p) w[j] = 0.0;
+        eq += x[j] == thr && x[j] != -INFINITY;
+      }
+      s += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    s = warp_sum_d(s);
+    eq = warp_sum_i(eq);
+    if (lane == 0) { sh.seg_sum[g] = s; sh.seg_tie[g] = eq; }
+  }
+  __syncthreads();
+  if (warp != 0) return;
   // the piece: 32 at a time, lane by lane
   double run = my_begin, sg_run = 0.0;
   int left = my_ties, sg = -1, sg_left = 0;
@@ -1133,7 +1323,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     const unsigned int eq = __ballot_sync(0xffffffffu, x == thr && x != -INFINITY);
     const int rank = __popc(eq & ((1u << lane) - 1u));
     double w = 0.0;
-    if (x > thr || (xmax - x) * scale < t_sure) { w = w_of(x); if (w < min_p) w = 0.0; }
+    if (x > thr || depth(x) < t_sure) { w = w_of(x); if (w < min_p) w = 0.0; }
     else if ((eq >> lane & 1u) && rank < left) w = w_tie;
     double s = w;
 #pragma unroll
