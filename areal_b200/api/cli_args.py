@@ -80,6 +80,7 @@ class GenerationHyperparameters:
     use_beam_search: bool = False
     reward_normalization: bool = False
     drop_incomplete_group: bool = False
+    min_p: float = 0.0                # tokens below this share of the likeliest one's probability are not drawn (0: off)
 
     def new(self, **kwargs) -> "GenerationHyperparameters":
         d = {f.name: copy.copy(getattr(self, f.name)) for f in fields(self)}
@@ -501,7 +502,12 @@ class NativeInferConfig:
     # KV pool in pausable memory (addresses survive while the physical pages leave the GPU): offload() then
     # really returns the pool's memory to the device and onload() takes it back without re-capturing CUDA graphs
     pausable_kv_cache: bool = False
+    # bfloat16, or float8_e4m3 (also fp8_e4m3): codes with a power-of-two scale for each page and head, half the bytes per decode step and
+    # twice the tokens in the pool; head sizes 64 and 128, models on the paged cache
     kv_cache_dtype: str = "bfloat16"
+    # Requests with top-k / top-p / min-p: "host" copies the step's logits and sorts them there, row by row (the draws of earlier versions);
+    # "device" samples them in one kernel, with draws of its own that depend on the request's seed and the position
+    filtered_sampling: str = "host"
     use_cuda_graph: bool = True
     compute_dtype: str = "bfloat16"  # float32: matrices, activations and cache in 32 bits (mixer stacks only)
     weight_dtype: str = "bfloat16"  # or float8_e4m3fn (block-scaled)

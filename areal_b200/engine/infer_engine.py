@@ -34,8 +34,10 @@ from ..api.engine_api import InferenceEngine
 from ..api.io_struct import ModelRequest, ModelResponse, ParamSpec, WeightUpdateMeta
 from ..models.config import ModelConfig
 from ..models.decoder import CausalLM, PackedBatch, build_model
+from ..ops import cache_ops as CO
 from ..ops import functional as OF
 from ..ops import lib as oplib
+from ..ops import sampling as OS
 from ..utils import logging as alog
 from .ragged_step import DECODE_BUCKETS, Entry, RaggedRunner
 from .state_cache import Carried, PagePool, StateCache
@@ -67,6 +69,7 @@ class _Seq:
     aborted: bool = False
     top_p: float = 1.0
     top_k: int = 0
+    min_p: float = 0.0
     stop_strs: tuple = ()                  # stop strings (need the request's tokenizer)
     tokenizer: Any = None
     stop_window: int = 16                  # tokens decoded per check
@@ -76,12 +79,22 @@ class _Seq:
     hstate: Any = None                     # recurrent-state models: models.hybrid.SequenceState once the prompt is absorbed
 
 
-class PagedKVCache(PagePool):
-    """K and V pages for all layers: ``[layers, 2, num_pages * page_size, Hkv, D]``."""
+EIGHT_BIT_CACHES = ("float8_e4m3", "float8_e4m3fn", "fp8_e4m3", "fp8")
+SIXTEEN_BIT_CACHES = ("bfloat16", "bf16", "auto", "")
 
-    def __init__(self, cfg: ModelConfig, num_pages: int, page_size: int, device, dtype, pausable: bool = False):
+
+class PagedKVCache(PagePool):
+    """K and V pages for all layers: ``[layers, 2, num_pages * page_size, Hkv, D]``; in 8 bits (``eight_bit``) codes
+    ``[layers, 2, num_pages, Hkv, page_size, D]`` as bytes and scales ``[layers, 2, num_pages, Hkv]`` (:class:`~areal_b200.ops.cache_ops.QuantPages`)."""
+
+    def __init__(self, cfg: ModelConfig, num_pages: int, page_size: int, device, dtype, pausable: bool = False, eight_bit: bool = False):
         super().__init__(num_pages, page_size)
-        shape = (cfg.num_layers, 2, num_pages * page_size, cfg.num_kv_heads, cfg.head_dim)
+        self.eight_bit = eight_bit
+        if eight_bit:
+            shape, dtype = (cfg.num_layers, 2, num_pages, cfg.num_kv_heads, page_size, cfg.head_dim), torch.uint8
+            self.scales = torch.zeros(cfg.num_layers, 2, num_pages, cfg.num_kv_heads, device=device)
+        else:
+            shape = (cfg.num_layers, 2, num_pages * page_size, cfg.num_kv_heads, cfg.head_dim)
         self.pausable = None
         if pausable:
             from ..ops import vmm
@@ -95,6 +108,24 @@ class PagedKVCache(PagePool):
                 self.data.zero_()
         if self.pausable is None:
             self.data = torch.zeros(*shape, device=device, dtype=dtype)
+
+    @staticmethod
+    def bytes_per_page(cfg: ModelConfig, page_size: int, eight_bit: bool = False) -> int:
+        rows = cfg.num_layers * 2 * cfg.num_kv_heads
+        return rows * (page_size * cfg.head_dim + 4) if eight_bit else rows * page_size * cfg.head_dim * 2
+
+    def layer(self, i: int) -> CO.QuantPages:
+        """The 8-bit pages of one layer."""
+        codes = self.data[i].view(CO.F8)
+        return CO.QuantPages(codes[0], codes[1], self.scales[i, 0], self.scales[i, 1])
+
+    def copy(self, src: list, dst: list, tokens: list) -> None:
+        """The first ``tokens[i]`` tokens of page ``src[i]`` to page ``dst[i]``, all layers, in one launch."""
+        if self.eight_bit:
+            CO.copy_pages([(self.data, 2, 4), (self.scales, 2, None)], src, dst, tokens)
+        else:
+            d = self.data
+            CO.copy_pages([(d.view(d.shape[0], 2, self.num_pages, self.page_size, *d.shape[3:]), 2, 3)], src, dst, tokens)
 
 
 class NativeInferenceEngine(InferenceEngine):
@@ -114,6 +145,8 @@ class NativeInferenceEngine(InferenceEngine):
         self._inbox: collections.deque = collections.deque()
         self.config = config or InferenceEngineConfig()
         self.icfg = infer_config or NativeInferConfig()
+        if self.icfg.filtered_sampling not in ("host", "device"):
+            raise ValueError(f"filtered_sampling is host or device, not {self.icfg.filtered_sampling!r}")
         self.model_config = model_config or (model.cfg if model is not None else None)
         self.model = model
         self.eos_token_id = eos_token_id
@@ -137,6 +170,8 @@ class NativeInferenceEngine(InferenceEngine):
         self.runner: Optional[RaggedRunner] = None
         self._ragged = False
         self._context_limit = self.icfg.context_length
+        self._filter_buf = None             # sampling filters of a step, pinned and on the device
+        self.eight_bit_cache = False
         self._sampled: list = []            # mixer stacks: requests whose sampling parameters the device buffers hold
 
     # ------------------------------------------------------------------ lifecycle
@@ -239,7 +274,13 @@ class NativeInferenceEngine(InferenceEngine):
         # trainer moved them into its flat buffer) would otherwise count as taken
         torch.cuda.empty_cache()
         free, total = torch.cuda.mem_get_info()
-        per_page = cfg.num_layers * 2 * ic.page_size * cfg.num_kv_heads * cfg.head_dim * 2
+        self.eight_bit_cache = ic.kv_cache_dtype in EIGHT_BIT_CACHES
+        if self.eight_bit_cache:
+            if cfg.head_dim not in (64, 128) or ic.page_size not in CO.PAGE_SIZES:
+                raise ValueError(f"an 8-bit cache takes head sizes of 64 and 128 and pages of {CO.PAGE_SIZES} tokens, not {cfg.head_dim} and {ic.page_size}")
+        elif ic.kv_cache_dtype not in SIXTEEN_BIT_CACHES:
+            logger.warning("kv_cache_dtype %r is not built: the cache is kept in bfloat16", ic.kv_cache_dtype)
+        per_page = PagedKVCache.bytes_per_page(cfg, ic.page_size, self.eight_bit_cache)
         if getattr(ic, "reserve_free_gb", 0.0) > 0:
             budget = free - int(ic.reserve_free_gb * (1 << 30))
         else:
@@ -249,7 +290,7 @@ class NativeInferenceEngine(InferenceEngine):
         if getattr(ic, "num_pages", None):
             n_pages = ic.num_pages
         self.cache = PagedKVCache(cfg, n_pages, ic.page_size, self.device, torch.bfloat16,
-                                  pausable=bool(getattr(ic, "pausable_kv_cache", False)))
+                                  pausable=bool(getattr(ic, "pausable_kv_cache", False)), eight_bit=self.eight_bit_cache)
         self.max_pages_per_seq = ic.context_length // ic.page_size + 1
         B = max(b for b in DECODE_BUCKETS if b <= max(1, ic.max_running_requests)) if ic.max_running_requests >= 1 else 1
         self.max_batch = B
@@ -469,7 +510,7 @@ class NativeInferenceEngine(InferenceEngine):
             return
         if self.cache is None and self.device.type == "cuda" and not self._recompute_decode:
             n, ps = self._saved_cache_shape
-            self.cache = PagedKVCache(self.model_config, n, ps, self.device, torch.bfloat16)
+            self.cache = PagedKVCache(self.model_config, n, ps, self.device, torch.bfloat16, eight_bit=self.eight_bit_cache)
         self.continue_generation()
 
     # ------------------------------------------------------------------ request API
@@ -532,7 +573,7 @@ class NativeInferenceEngine(InferenceEngine):
                        # a request without its own seed: its id hashed with the engine's seed (``native_infer.random_seed``)
                        seed=(g.seed if g.seed is not None else zlib.crc32(req.rid.encode()) ^ (int(self.icfg.random_seed) * 0x9E3779B1)) & 0x7FFFFFFF,
                        future=(loop, fut),
-                       t_submit=time.perf_counter(), top_p=g.top_p, top_k=0 if g.top_k >= 10 ** 7 else int(g.top_k),
+                       t_submit=time.perf_counter(), top_p=g.top_p, min_p=g.min_p, top_k=0 if g.top_k >= 10 ** 7 else int(g.top_k),
                        mm=mm, rope_delta=rope_delta, stop_strs=tuple(g.stop or ()), tokenizer=getattr(req, "tokenizer", None),
                        stop_window=max(8, 2 * max((len(x) for x in (g.stop or [""])), default=0)))
             with self._lock:
@@ -625,7 +666,7 @@ class NativeInferenceEngine(InferenceEngine):
             self._idle.set()
 
     _SEQ_WIRE_FIELDS = ("rid", "tokens", "prompt_len", "max_new", "min_new", "temperature", "greedy", "stop_ids", "ignore_eos", "seed",
-                        "top_p", "top_k", "rope_delta")
+                        "top_p", "top_k", "min_p", "rope_delta")
 
     def _tp_sync_control(self, paused: bool):
         """One exchange per loop iteration of a tensor-parallel replica: every rank reports its
@@ -813,7 +854,7 @@ class NativeInferenceEngine(InferenceEngine):
         done: list = []
         if ready:
             if self.device.type == "cuda":
-                if ready == self._sampled and all(s.top_p >= 1.0 and s.top_k <= 0 for s in ready):
+                if ready == self._sampled and all(_plain(s) for s in ready):
                     # the rows of the step before: their sampling parameters are on the device
                     self._sample_rows(logits, len(ready), self.s_inv_temp, self.s_greedy, self.s_seeds)
                     toks, lps = self._fetch_samples(len(ready))
@@ -853,6 +894,8 @@ class NativeInferenceEngine(InferenceEngine):
             return tok, float(lp_all[tok])
         z = logits.float() / max(s.temperature, 1e-6)
         z = _apply_top_k_top_p(z, s.top_k, s.top_p)
+        if s.min_p > 0:
+            z = torch.where(torch.exp(z - z.max()) < min(s.min_p, 1.0), torch.full_like(z, float("-inf")), z)
         lp_all = torch.log_softmax(z, -1)
         gen = torch.Generator().manual_seed((s.seed * 1000003 + len(s.tokens)) & 0x7FFFFFFF)
         tok = int(torch.multinomial(lp_all.exp(), 1, generator=gen))
@@ -953,6 +996,17 @@ class NativeInferenceEngine(InferenceEngine):
         fns = []
         scale = 1.0 / math.sqrt(cfg.head_dim)
         L = oplib.get_lib()
+        if self.cache.eight_bit:
+            for li in range(cfg.num_layers):
+                def fn(q, k, v, pages=self.cache.layer(li)):
+                    if mode == "prefill":
+                        CO.kv8_append(k, v, pages, kw["pt"], kw["lens"], kw["seq_cu"])
+                        o, _ = OF.attention_fwd(q, k, v, kw["cu"], True, scale, kw["tile_info"])
+                        return o
+                    CO.kv8_append(k, v, pages, kw["pt"], kw["lens"])
+                    return CO.kv8_decode(q, pages, kw["pt"], kw["lens"], scale)
+                fns.append(fn)
+            return fns
         for li in range(cfg.num_layers):
             kc, vc = self.cache.data[li, 0], self.cache.data[li, 1]
 
@@ -1062,7 +1116,7 @@ class NativeInferenceEngine(InferenceEngine):
                 return
             tail_page = got[0]
             src = s.pages[n_full]
-            self.cache.data[:, :, tail_page * ps: tail_page * ps + tail] = self.cache.data[:, :, src * ps: src * ps + tail]
+            self.cache.copy([src], [tail_page], [tail])
         full = list(s.pages[:n_full])
         self.cache.share(full)
         self._prefix[key] = dict(pages=full, tail_page=tail_page, tail=tail, n=n, logits=logits_row.clone(), version=self._version)
@@ -1073,6 +1127,7 @@ class NativeInferenceEngine(InferenceEngine):
         started; the others (entry evicted since admission) are back at the head of the waiting queue."""
         ps = self.cache.page_size
         ready, rows = [], []
+        src, dst, tails = [], [], []
         for s, key in reuse:
             ent = self._prefix_lookup(key)
             if ent is None:                            # the sequence that was to prefetch it did not get to (eviction, failure)
@@ -1085,13 +1140,16 @@ class NativeInferenceEngine(InferenceEngine):
             self.cache.share(ent["pages"])
             s.pages = list(ent["pages"]) + private
             if ent["tail"]:
-                dst, src = private[0], ent["tail_page"]
-                self.cache.data[:, :, dst * ps: dst * ps + ent["tail"]] = self.cache.data[:, :, src * ps: src * ps + ent["tail"]]
+                src.append(ent["tail_page"])
+                dst.append(private[0])
+                tails.append(ent["tail"])
             s.cached = ent["n"]
             ready.append(s)
             rows.append(ent["logits"])
         if not ready:
             return ready
+        if src:
+            self.cache.copy(src, dst, tails)        # all of the group's forks in one launch
         toks, lps = self._sample_cuda(torch.stack(rows), ready)
         self.stats["prefix_hits"] += len(ready)
         self.stats["prefix_tokens_saved"] += sum(s.cached for s in ready)
@@ -1122,7 +1180,14 @@ class NativeInferenceEngine(InferenceEngine):
         cu = torch.tensor(cu_list, dtype=torch.int32)
         ids, pos, slots, cu = (t.pin_memory().to(dev, non_blocking=True) for t in (ids, pos, slots, cu))
         pb = PackedBatch(cu, pos, Tp, max(lens))
-        fns = self._layer_attn_fns("prefill", slots=slots, cu=cu, tile_info=pb.tile_info)
+        extra = {}
+        if self.cache.eight_bit:
+            table = torch.zeros(len(seqs), max(len(s.pages) for s in seqs), dtype=torch.int32)
+            for i, s in enumerate(seqs):
+                table[i, :len(s.pages)] = torch.tensor(s.pages, dtype=torch.int32)
+            table, lens_d = (t.pin_memory().to(dev, non_blocking=True) for t in (table, torch.tensor(lens, dtype=torch.int32)))
+            extra = dict(pt=table, lens=lens_d, seq_cu=cu[:len(seqs) + 1])
+        fns = self._layer_attn_fns("prefill", slots=slots, cu=cu, tile_info=pb.tile_info, **extra)
         if any(s.mm is not None for s in seqs):
             from ..models.vlm import collect_multi_modal
 
@@ -1160,11 +1225,34 @@ class NativeInferenceEngine(InferenceEngine):
         self._err_poll.check("rollout engine step")
         return self.hn_out_tok[:n].tolist(), self.hn_out_lp[:n].tolist()
 
+    def _sample_filtered(self, logits: torch.Tensor, n: int, rows: list):
+        """Top-k / top-p / min-p sampling on the device for ``rows`` ``[(row of logits, sequence)]`` out of ``n``. The number drawn for a token
+        depends on the request's seed and the token's position alone."""
+        self._step += 1
+        if self._filter_buf is None or self._filter_buf[0].shape[1] < n:
+            size = max(n, self.max_batch)
+            self._filter_buf = torch.zeros(6, size, dtype=torch.int32).pin_memory(), torch.zeros(6, size, dtype=torch.int32, device=self.device)
+        host, dev = self._filter_buf
+        h = host.numpy()
+        f = h.view(np.float32)
+        h[:, :n] = 0
+        h[0, :n] = 1                                     # rows without a request: greedy, whatever their logits are
+        f[2, :n] = f[4, :n] = 1.0
+        for r, s in rows:
+            h[0, r], h[1, r] = int(s.greedy), s.top_k
+            f[2, r] = 1.0 if s.greedy else 1.0 / max(s.temperature, 1e-6)
+            f[3, r], f[4, r], f[5, r] = _uniform01(s.seed, len(s.tokens)), s.top_p, s.min_p
+        dev.copy_(host, non_blocking=True)
+        fl = dev.view(torch.float32)
+        OS.sample_filtered(logits, fl[3, :n], fl[2, :n], dev[1, :n], fl[4, :n], fl[5, :n], dev[0, :n], out=(self.s_out_tok[:n], self.s_out_lp[:n]))
+        return self._fetch_samples(n)
+
     def _sample_cuda(self, logits: torch.Tensor, seqs: list[_Seq]):
         """Sampling for an ad-hoc list of sequences (prefill path)."""
         n = len(seqs)
-        plain = all(s.top_p >= 1.0 and s.top_k <= 0 for s in seqs)
-        if not plain:
+        if not all(_plain(s) for s in seqs):
+            if self.icfg.filtered_sampling == "device":
+                return self._sample_filtered(logits, n, list(enumerate(seqs)))
             self._step += 1
             out_t, out_l = [], []
             lg = logits.float().cpu()
@@ -1256,14 +1344,15 @@ class NativeInferenceEngine(InferenceEngine):
             oplib.LAUNCHES["count"] += n_kernels
         else:
             logits = self._decode_forward(B)
-        plain = all(s.top_p >= 1.0 and s.top_k <= 0 for s in seqs)
-        if plain:
+        if all(_plain(s) for s in seqs):
             st = self.d_state
             self.s_greedy[:B].copy_(st[:B, 4])
             self.s_seeds[:B].copy_(st[:B, 5])
             self.s_inv_temp[:B].copy_(st[:B, 6].view(torch.float32))
             self._sample_rows(logits, B, self.s_inv_temp, self.s_greedy, self.s_seeds)
             toks, lps = self._fetch_samples(B)
+        elif self.icfg.filtered_sampling == "device":
+            toks, lps = self._sample_filtered(logits[:B], B, [(s.row, s) for s in seqs])
         else:
             self._step += 1
             lg = logits[:B].float().cpu()
@@ -1298,6 +1387,19 @@ class NativeInferenceEngine(InferenceEngine):
         out = {f"infer/{k}": float(v) for k, v in self.stats.items()}
         out["infer/alive_seconds"] = time.perf_counter() - self._t_start
         return out
+
+
+def _plain(s: _Seq) -> bool:
+    """No filter but the temperature."""
+    return s.top_p >= 1.0 and s.top_k <= 0 and s.min_p <= 0.0
+
+
+def _uniform01(seed: int, position: int) -> float:
+    """A number in [0, 1) with 24 bits for one token of one request (SplitMix64 of both)."""
+    z = (seed * 0x9E3779B97F4A7C15 + (position + 1) * 0xD1342543DE82EF95) & 0xFFFFFFFFFFFFFFFF
+    z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & 0xFFFFFFFFFFFFFFFF
+    z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & 0xFFFFFFFFFFFFFFFF
+    return ((z ^ (z >> 31)) >> 40) / float(1 << 24)
 
 
 def _apply_top_k_top_p(z: torch.Tensor, top_k: int, top_p: float) -> torch.Tensor:

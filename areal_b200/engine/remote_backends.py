@@ -37,9 +37,12 @@ class GenerationResult:
 
 
 def _sampling(g, budget: int, done: int) -> dict:
-    return {"max_new_tokens": budget - done, "min_new_tokens": max(0, g.min_new_tokens - done),
-            "temperature": 0.0 if g.greedy else g.temperature, "top_p": g.top_p,
-            "top_k": -1 if g.top_k >= 10 ** 7 else g.top_k, "stop_token_ids": g.stop_token_ids, "ignore_eos": g.ignore_eos}
+    p = {"max_new_tokens": budget - done, "min_new_tokens": max(0, g.min_new_tokens - done),
+         "temperature": 0.0 if g.greedy else g.temperature, "top_p": g.top_p,
+         "top_k": -1 if g.top_k >= 10 ** 7 else g.top_k, "stop_token_ids": g.stop_token_ids, "ignore_eos": g.ignore_eos}
+    if getattr(g, "min_p", 0.0) > 0:
+        p["min_p"] = g.min_p
+    return p
 
 
 class NativeBackend:
@@ -109,6 +112,8 @@ class VLLMBackend(NativeBackend):
              "temperature": 0.0 if g.greedy else g.temperature, "top_p": g.top_p, "top_k": -1 if g.top_k >= 10 ** 7 else g.top_k,
              "stop_token_ids": g.stop_token_ids, "ignore_eos": g.ignore_eos, "frequency_penalty": getattr(g, "frequency_penalty", 0.0),
              "return_tokens_as_token_ids": True, "logprobs": 0, "stream": False, "request_id": rid}
+        if getattr(g, "min_p", 0.0) > 0:
+            p["min_p"] = g.min_p
         if getattr(g, "stop", None):
             p["stop"] = list(g.stop)
         if g.seed is not None:

@@ -40,7 +40,7 @@ def gconfig_from_sampling_params(sp: dict) -> GenerationHyperparameters:
         n_samples=1, max_new_tokens=int(sp.get("max_new_tokens", 128)), min_new_tokens=int(sp.get("min_new_tokens", 0)),
         max_tokens=int(sp.get("max_tokens", 1 << 30)), greedy=t == 0.0 or bool(sp.get("greedy", False)), temperature=t if t > 0 else 1.0,
         top_p=float(sp.get("top_p", 1.0)), top_k=int(sp.get("top_k", -1)) if int(sp.get("top_k", -1)) > 0 else int(1e8),
-        stop_token_ids=list(sp.get("stop_token_ids") or []), ignore_eos=bool(sp.get("ignore_eos", False)),
+        min_p=float(sp.get("min_p", 0.0)), stop_token_ids=list(sp.get("stop_token_ids") or []), ignore_eos=bool(sp.get("ignore_eos", False)),
         seed=sp.get("seed"))
 
 
