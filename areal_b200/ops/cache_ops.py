@@ -16,7 +16,6 @@ import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 
 from . import lib as _lib
@@ -206,17 +205,20 @@ def _decode_workspace(dev: int, *sizes: int) -> tuple[int, int]:
         return int(_lib.get_lib().ab2_kv8_decode_workspace(*sizes, ctypes.addressof(n))), n.value
 
 
-_COUNTERS: dict = {}        # (device, stream) -> zeros that every call on the stream leaves zero
+_SCRATCH: dict = {}         # (device, stream) -> (counters, workspace) of the calls on that stream
 
 
-def _counters(dev: int, n: int) -> torch.Tensor:
-    """Zeros that calls on the current stream may share, one after the other; a captured call gets its own, cleared in its graph."""
+def _scratch(dev: int, size: int, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(``n`` counters, a workspace of ``size`` bytes). Calls on one stream run one after the other and share them: every call leaves the
+    counters zero and reads of the workspace only what it has written. A captured call gets its own, the counters cleared in its graph."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.int32, device=f"cuda:{dev}")
+        return torch.zeros(n, dtype=torch.int32, device=f"cuda:{dev}"), torch.empty(size, dtype=torch.uint8, device=f"cuda:{dev}")
     key = dev, torch._C._cuda_getCurrentRawStream(dev)
-    c = _COUNTERS.get(key)
-    if c is None or c.numel() < n:
-        c = _COUNTERS[key] = torch.zeros(max(n, 1024), dtype=torch.int32, device=f"cuda:{dev}")
+    c = _SCRATCH.get(key)
+    if c is None or c[0].numel() < n or c[1].numel() < size:
+        old = (0, 0) if c is None else (c[0].numel(), c[1].numel())
+        c = _SCRATCH[key] = (torch.zeros(max(n, old[0], 1024), dtype=torch.int32, device=f"cuda:{dev}"),
+                             torch.empty(max(size, old[1]), dtype=torch.uint8, device=f"cuda:{dev}"))
     return c
 
 
@@ -227,8 +229,8 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     ``q`` ``[B, Hq, D]`` bf16, heads dense, rows a multiple of 8 elements apart (the query part of a wider projection); ``Hq`` a multiple of the cache's
     heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous, where given);
     a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
-    length beyond the table, sets the device error word (code 6); the row's result is not to be used. The workspace is allocated in
-    the call, and the counters belong to the stream or, in a captured call, to its graph: calls on several streams and graphs share neither. At most
+    length beyond the table, sets the device error word (code 6); the row's result is not to be used. Workspace and
+    counters belong to the current stream or, in a captured call, to its graph: calls on several streams and graphs share neither. At most
     8192 sequences."""
     shape = q.shape
     if not (len(shape) == 3 and q.dtype is torch.bfloat16):
@@ -257,10 +259,9 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
         raise ValueError("heads of a row have to be dense")
     if row & 7 or q.data_ptr() & 15:
         raise ValueError("rows have to start on 16 bytes")
-    size, n = _decode_workspace(dev, B, Hq, Hkv, D, ps, width)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    counters, ws = _scratch(dev, *_decode_workspace(dev, B, Hq, Hkv, D, ps, width))
     _launch(dev, "ab2_kv8_decode", q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
-            page_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), _counters(dev, n).data_ptr(), B, Hq, Hkv, D, ps, width, P, scale, row)
+            page_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), counters.data_ptr(), B, Hq, Hkv, D, ps, width, P, scale, row)
     return out
 
 
@@ -285,46 +286,59 @@ def copy_pages(buffers: Sequence[tuple], src, dst, tokens=None) -> None:
     ``src``, ``dst``, ``tokens``: host sequences of ints or integer arrays; ``tokens[i]`` leading tokens of page i are copied, the rest of the
     destination stays as it is (None: whole pages). A source may stand for several destinations; no page may be a destination twice, or source and
     destination at once."""
-    src, dst = np.asarray(src, np.int32).reshape(-1), np.asarray(dst, np.int32).reshape(-1)
+    src, dst = _ints(src), _ints(dst)
     n = len(src)
-    _need(len(dst) == n and 0 < len(buffers) <= 4, "one destination for each source, one to four buffers")
-    dev, pages, slots = buffers[0][0].device, None, None
+    if len(dst) != n or not 0 < len(buffers) <= 4:
+        raise ValueError("one destination for each source, one to four buffers")
+    dev, pages, slots = buffers[0][0].get_device(), None, None
     desc = []
     for t, page_dim, token_dim in buffers:
-        shape = t.shape
-        _need(t.device == dev and t.is_contiguous() and t.numel() > 0, "buffers: contiguous, on one device")
-        _need(0 <= page_dim < len(shape) and (token_dim is None or page_dim < token_dim < len(shape)), "no such dims")
-        _need(pages in (None, shape[page_dim]), "buffers of different numbers of pages")
-        pages = shape[page_dim]
-        if token_dim is not None:
-            _need(slots in (None, shape[token_dim]), "buffers of different page sizes")
-            slots = shape[token_dim]
-        st, es = t.stride(), t.element_size()
-        planes = t.numel() // (pages * st[page_dim])
+        shape, st, es = t.shape, t.stride(), t.element_size()
+        if not (t.get_device() == dev and t.is_contiguous() and t.numel() > 0):
+            raise ValueError("buffers: contiguous, on one device")
+        if not (0 <= page_dim < len(shape) and (token_dim is None or page_dim < token_dim < len(shape))):
+            raise ValueError("no such dims")
+        p = shape[page_dim]
+        if pages is None:
+            pages = p
+        elif pages != p:
+            raise ValueError("buffers of different numbers of pages")
         whole = st[page_dim] * es
-        if tokens is None or token_dim is None:
-            rows, row, tok = 1, whole, 0
-        else:
-            tok = st[token_dim] * es
-            row = tok * shape[token_dim]
-            rows = whole // row
-        _need(whole < (1 << 31) - (1 << 14), "a page of 2 GB")
-        desc += [t.data_ptr(), whole * pages, whole, row, planes, rows, row, tok, pages, 0]
+        rows, row, tok = 1, whole, 0
+        if token_dim is not None:
+            if slots is None:
+                slots = shape[token_dim]
+            elif slots != shape[token_dim]:
+                raise ValueError("buffers of different page sizes")
+            if tokens is not None:
+                tok = st[token_dim] * es
+                row = tok * slots
+                rows = whole // row
+        if whole >= (1 << 31) - (1 << 15):
+            raise ValueError("a page of 2 GB")
+        desc += (t.data_ptr(), whole * p, whole, row, t.numel() * es // (whole * p), rows, row, tok, p, 0)
     if n == 0:
         return
-    _need(int(src.min()) >= 0 and int(src.max()) < pages and int(dst.min()) >= 0 and int(dst.max()) < pages, f"pages outside of 0 .. {pages - 1}")
-    to = set(dst.tolist())
-    _need(len(to) == n, "a page is the destination of two copies")
-    _need(to.isdisjoint(src.tolist()), "a page is source and destination")
+    to = set(dst)
+    if min(src) < 0 or max(src) >= pages or min(dst) < 0 or max(dst) >= pages:
+        raise ValueError(f"pages outside of 0 .. {pages - 1}")
+    if len(to) != n:
+        raise ValueError("a page is the destination of two copies")
+    if not to.isdisjoint(src):
+        raise ValueError("a page is source and destination")
     if tokens is not None:
-        tokens = np.asarray(tokens, np.int32).reshape(-1)
-        _need(len(tokens) == n and slots is not None and int(tokens.min()) >= 0 and int(tokens.max()) <= slots, "tokens: 0 to the page size, one for each pair")
-    if not dev.type == "cuda":
+        tokens = _ints(tokens)
+        if not (len(tokens) == n and slots is not None and min(tokens) >= 0 and max(tokens) <= slots):
+            raise ValueError("tokens: 0 to the page size, one for each pair")
+    if dev < 0:
         return copy_pages_ref(buffers, src, dst, tokens)
-    pairs = np.empty((n, 3), np.int32)
-    pairs[:, 0], pairs[:, 1], pairs[:, 2] = src, dst, -1 if tokens is None else tokens
-    flat = (ctypes.c_longlong * len(desc))(*desc)
-    _launch(dev.index, "ab2_copy_pages", ctypes.addressof(flat), len(buffers), pairs.ctypes.data, n)
+    pairs = src + dst + (tokens if tokens is not None else [-1] * n)
+    flat, args = (ctypes.c_longlong * len(desc))(*desc), (ctypes.c_int * (3 * n))(*pairs)
+    _launch(dev, "ab2_copy_pages", ctypes.addressof(flat), len(buffers), ctypes.addressof(args), n)
+
+
+def _ints(x) -> list:
+    return x.tolist() if hasattr(x, "tolist") else list(x)
 
 
 _lib.declare("ab2_kv8_append", [_V] * 9 + [_I] * 7 + [_L, _L, _V])

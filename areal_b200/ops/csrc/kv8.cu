@@ -28,16 +28,21 @@ __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a < INFINITY ? a : 0.f;                       // infinities saturate and NaN stays NaN: neither sets a scale
 }
-__device__ __forceinline__ float amax8(const uint4& v) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  float a = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack_bf16(w[i]);
-    a = fmaxf(a, fmaxf(finite_abs(f.x), finite_abs(f.y)));
-  }
-  return a;
+// Sizes of bf16 numbers order as their bits do without the sign: two at a time in one word.
+__device__ __forceinline__ uint32_t size2(uint32_t a, uint32_t w) {
+  uint32_t r;
+  asm("max.s16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(w & 0x7fff7fffu));
+  return r;
 }
+__device__ __forceinline__ uint32_t size8(uint32_t a, const uint4& v) { return size2(size2(size2(size2(a, v.x), v.y), v.z), v.w); }
+// The same without infinities and NaN, for the rare rows that hold any.
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  const uint32_t lo = w & 0x7fffu, hi = w & 0x7fff0000u;
+  return (lo < 0x7f80u ? lo : 0u) | (hi < 0x7f800000u ? hi : 0u);
+}
+__device__ __forceinline__ float larger_half(uint32_t a) { return __uint_as_float(max(a << 16, a & 0xffff0000u)); }
+constexpr uint32_t BF16_INF = 0x7f800000u;
+
 __device__ __forceinline__ uint32_t code4(uint32_t lo, uint32_t hi, float inv) {
   const float2 a = unpack_bf16(lo), b = unpack_bf16(hi);
   const uint32_t c0 = __nv_cvt_float2_to_fp8x2(make_float2(a.x * inv, a.y * inv), __NV_SATFINITE, __NV_E4M3);
@@ -78,7 +83,7 @@ struct Kv8Args {
 // row, one of the scale, one store of each; a warp re-codes its block (8 KB at 64 x 128) only when the scale grows.
 template <int D>
 __global__ void __launch_bounds__(128)
-kv8_append_row_kernel(Kv8Args a, const int* __restrict__ table, const int* __restrict__ lens, int B, int Hkv, int page_size, int width,
+kv8_append_row_kernel(const __grid_constant__ Kv8Args a, const int* __restrict__ table, const int* __restrict__ lens, int B, int Hkv, int page_size, int width,
                       int num_pages, int* __restrict__ err) {
   pdl_wait();
   pdl_trigger();
@@ -131,46 +136,60 @@ kv8_append_row_kernel(Kv8Args a, const int* __restrict__ table, const int* __res
 // in one contiguous run. Which page a block has: the pages of sequence b are numbered from cu[b] / page_size + 2 b on, which
 // leaves room for the floor(n / page_size) + 2 that n rows can touch, so no scan over the batch is needed.
 template <int D, int NV>          // NV: 16-byte pieces of a thread = page_size * D / 8 / 128
-__global__ void __launch_bounds__(128)
-kv8_append_page_kernel(Kv8Args a, const int* __restrict__ table, const int* __restrict__ lens, const int* __restrict__ cu, int B, int rows,
+__global__ void __launch_bounds__(128, NV <= 8 ? 8 : 4)
+kv8_append_page_kernel(const __grid_constant__ Kv8Args a, const int* __restrict__ table, const int* __restrict__ lens, const int* __restrict__ cu, int B, int rows,
                        int Hkv, int page_size, int width, int num_pages, int* __restrict__ err) {
   __shared__ float red[4];
+  __shared__ int found[4];             // of this block's sequence: first row, first row of the next, length
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, item = blockIdx.x, h = blockIdx.y >> 1, kv = blockIdx.y & 1;
   int b = -1;
-  for (int i0 = 0; i0 < B; i0 += 128) {                // numbers grow with b: how many do not pass this block's
-    const int i = i0 + tid;
-    const int n = __syncthreads_count(i < B && cu[min(i, B - 1)] / page_size + 2 * i <= item);
+  for (int i0 = 0; i0 < B; i0 += 128) {                // numbers grow with b: the last one that does not pass this block's
+    const int i = i0 + tid, k = min(i, B - 1);
+    const int c = cu[k], next = cu[k + 1], len = lens[k];
+    const int n = __syncthreads_count(i < B && c / page_size + 2 * i <= item);
+    if (n && tid == n - 1) { found[0] = c; found[1] = next; found[2] = len; }
     b += n;
     if (n < 128) break;
   }
+  __syncthreads();
   if (b < 0) return;
-  const int c0 = cu[b], n = cu[b + 1] - c0, end = lens[b], start = end - n;
+  const int c0 = found[0], n = found[1] - c0, end = found[2], start = end - n;
   if (n <= 0) return;
   const int j = start / page_size + item - (c0 / page_size + 2 * b);
   const int lo = max(start, j * page_size), hi = min(end, (j + 1) * page_size);
   if (start >= 0 && lo >= hi) return;
-  const int page = start >= 0 && j < width && c0 >= 0 && c0 + n <= rows ? table[(size_t)b * width + j] : -1;
-  if (page < 0 || page >= num_pages) {
-    if (tid == 0) set_error(err, ERR_BOUNDS);
-    return;
-  }
-  const size_t blk = (size_t)page * Hkv + h;
-  const int slot = lo - j * page_size, cnt = hi - lo;
-  float* scale = kv ? a.scales[1] : a.scales[0];
-  const float old = slot ? scale[blk] : 0.f;
+  const bool fits = start >= 0 && j < width && c0 >= 0 && c0 + n <= rows;
+  // the rows do not need the page's number: they are on their way while it is looked up
+  const int page = fits ? table[(size_t)b * width + j] : -1;
+  const int slot = lo - j * page_size, cnt = fits ? hi - lo : 0;
   const long long stride = kv ? a.stride[1] : a.stride[0];
-  const __nv_bfloat16* x = (kv ? a.x[1] : a.x[0]) + (size_t)(c0 + lo - start) * stride + h * D;
+  const __nv_bfloat16* x = (kv ? a.x[1] : a.x[0]) + (fits ? (size_t)(c0 + lo - start) * stride + h * D : 0);
   uint4 v[NV];
-  float m = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int p = tid + i * 128, row = p / (D / 8), piece = p % (D / 8);
     v[i] = row < cnt ? *reinterpret_cast<const uint4*>(x + row * stride + piece * 8) : make_uint4(0u, 0u, 0u, 0u);
   }
+  if (page < 0 || page >= num_pages) {
+    if (tid == 0) set_error(err, ERR_BOUNDS);
+    return;
+  }
+  const size_t blk = (size_t)page * Hkv + h;
+  float* scale = kv ? a.scales[1] : a.scales[0];
+  const float old = slot ? scale[blk] : 0.f;
+  uint32_t most = 0u;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) m = fmaxf(m, amax8(v[i]));
+  for (int i = 0; i < NV; ++i) most = size8(most, v[i]);
+  float m = larger_half(most);
+  if (__float_as_uint(m) >= BF16_INF) {
+    most = 0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      most = size2(size2(size2(size2(most, finite2(v[i].x)), finite2(v[i].y)), finite2(v[i].z)), finite2(v[i].w));
+    m = larger_half(most);
+  }
   m = warp_max(m);
   if ((tid & 31) == 0) red[tid >> 5] = m;
   __syncthreads();
@@ -664,12 +683,13 @@ static int launch_kv8_decode(const Kv8Decode& a, int grid, cudaStream_t s) {
 // ------------------------------------------------------------------ page copies
 // Copies pages src -> dst of up to four buffers in one launch: all planes (layers, keys and values, scales) of all pairs. A page of
 // a plane is `rows` runs of bytes, `row_stride` apart, of which the first tokens * token_bytes of each are copied (all of them where
-// tokens < 0). The pairs travel as kernel arguments, so a call needs no transfer. Bound by memory: 16 KB a block, 64 bytes a thread in flight.
-constexpr int COPY_PAIRS = 256, COPY_BUFFERS = 4, COPY_BYTES = 16384;
+// tokens < 0). The pairs travel as kernel arguments, so a call needs no transfer. Bound by memory: 16 KB a block, 64 bytes a thread in flight
+// (32 KB and 128 bytes cost 15 % where the runs do not fill the blocks, and gain nothing on whole pages).
+constexpr int COPY_PAIRS = 256, COPY_BUFFERS = 4, COPY_PER = 4, COPY_BYTES = 256 * 16 * COPY_PER;
 struct CopyBuffer {
   unsigned char* base;
   long long plane_stride, page_stride, row_stride;
-  int planes, rows, row_bytes, token_bytes, first_block, unit;     // unit: bytes of one access (16, 4 or 1)
+  int planes, rows, row_bytes, token_bytes, first_block, per, unit;     // per: blocks of one plane; unit: bytes of one access (16, 4 or 1)
 };
 struct CopyArgs {
   CopyBuffer buf[COPY_BUFFERS];
@@ -678,7 +698,7 @@ struct CopyArgs {
 };
 template <typename T>
 __device__ __forceinline__ void copy_run(const unsigned char* s, unsigned char* d, int run, long long row_stride, int first, int last) {
-  constexpr int U = sizeof(T), PER = 4;
+  constexpr int U = sizeof(T), PER = COPY_PER;
   for (int i0 = first / U + threadIdx.x; i0 < last / U; i0 += PER * 256) {
     T v[PER];
     long long off[PER];
@@ -705,8 +725,7 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
   for (int i = 1; i < COPY_BUFFERS; ++i)
     if (i < a.n_buf && (int)blockIdx.x >= a.buf[i].first_block) n = i;
   const CopyBuffer& c = a.buf[n];
-  const int per = (int)(((long long)c.rows * c.row_bytes + COPY_BYTES - 1) / COPY_BYTES);      // blocks of one plane
-  const int k = blockIdx.x - c.first_block, plane = k / per, part = k - plane * per;
+  const int k = blockIdx.x - c.first_block, plane = k / c.per, part = k - plane * c.per;
   if (plane >= c.planes) return;
   const int tok = a.tokens[pair];
   const int run = tok < 0 || c.token_bytes == 0 ? c.row_bytes : tok * c.token_bytes;
@@ -749,6 +768,7 @@ int ab2_kv8_append(const void* k, const void* v, void* kc, void* vc, void* ks, v
     else launch_pdl(kv8_append_row_kernel<64>, grid, dim3(128), 0, s, a, table, lens, B, Hkv, page_size, width, num_pages, err);
     return cudaGetLastError() == cudaSuccess ? 0 : 1;
   }
+  if (rows / page_size + 2LL * B > 0x7fffffffLL || Hkv * 2 > 65535) return 10;
   const dim3 grid(rows / page_size + 2 * B, Hkv * 2);
 #define AB2_APPEND(DD, NN) launch_pdl(kv8_append_page_kernel<DD, NN>, grid, dim3(128), 0, s, a, table, lens, cu, B, rows, Hkv, page_size, width, num_pages, err)
   switch (page_size * D / 1024) {
@@ -809,7 +829,7 @@ int ab2_kv8_decode(const void* q, const void* kc, const void* vc, const void* ks
 }
 
 // n_buf buffers, each ten values in `desc`: address, plane, page and row strides in bytes, planes, rows, bytes of a row, bytes of a token in a
-// row, pages, 0. pairs: src, dst, tokens of n pairs (host memory), tokens < 0 = whole page. No page may be both source and destination, or
+// row, pages, 0. pairs: n sources, n destinations, n numbers of tokens (host memory; < 0: whole page). No page may be both source and destination, or
 // destination twice: the caller has checked it.
 int ab2_copy_pages(const long long* desc, int n_buf, const int* pairs, int n, void* stream) {
   if (n <= 0 || n_buf <= 0) return 0;
@@ -817,6 +837,12 @@ int ab2_copy_pages(const long long* desc, int n_buf, const int* pairs, int n, vo
   CopyArgs a;
   a.n_buf = n_buf;
   long long blocks = 0;
+  int longest = 0;                                     // tokens of the longest copy; -1: whole pages
+  for (int i = 0; i < n; ++i) {
+    const int t = pairs[2 * n + i];
+    if (t < 0) { longest = -1; break; }
+    longest = t > longest ? t : longest;
+  }
   for (int i = 0; i < n_buf; ++i) {
     const long long* d = desc + 10 * i;
     CopyBuffer& c = a.buf[i];
@@ -825,15 +851,24 @@ int ab2_copy_pages(const long long* desc, int n_buf, const int* pairs, int n, vo
     c.plane_stride = d[1]; c.page_stride = d[2]; c.row_stride = d[3];
     c.planes = (int)d[4]; c.rows = (int)d[5]; c.row_bytes = (int)d[6]; c.token_bytes = (int)d[7];
     c.first_block = (int)blocks;
+    if (c.rows == 1 && c.token_bytes == 0 && c.row_bytes <= COPY_BYTES / 8) {       // a few bytes in each plane (scales): planes as rows
+      c.rows = c.planes;
+      c.planes = 1;
+      c.row_stride = c.plane_stride;
+      if ((long long)c.rows * c.row_bytes > 0x7fffffffLL - COPY_BYTES) return 10;
+    }
+    const long long most = c.token_bytes && longest >= 0 ? (long long)longest * c.token_bytes : c.row_bytes;
+    c.per = (int)((most * c.rows + COPY_BYTES - 1) / COPY_BYTES);
+    if (c.per < 1) c.per = 1;
     const long long all = d[0] | d[1] | d[2] | d[3] | d[6] | d[7];
     c.unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
-    blocks += (d[6] * d[5] + COPY_BYTES - 1) / COPY_BYTES * d[4];
+    blocks += (long long)c.per * c.planes;
     if (blocks > 0x7fffffffLL) return 10;
   }
   for (int at = 0; at < n; at += COPY_PAIRS) {
     const int m = n - at < COPY_PAIRS ? n - at : COPY_PAIRS;
     for (int i = 0; i < m; ++i) {
-      a.src[i] = pairs[3 * (at + i)]; a.dst[i] = pairs[3 * (at + i) + 1]; a.tokens[i] = pairs[3 * (at + i) + 2];
+      a.src[i] = pairs[at + i]; a.dst[i] = pairs[n + at + i]; a.tokens[i] = pairs[2 * n + at + i];
     }
     launch_pdl(copy_pages_kernel, dim3((unsigned)blocks, m), dim3(256), 0, (cudaStream_t)stream, a);
   }
