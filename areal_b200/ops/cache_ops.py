@@ -198,27 +198,23 @@ def kv8_decode_ref(q, pages: QuantPages, page_table, seq_lens, scale: Optional[f
 
 
 @functools.lru_cache(maxsize=256)
-def _decode_workspace(dev: int, *sizes: int) -> tuple[int, int]:
-    """(bytes of the workspace, number of counters) for these sizes."""
-    n = ctypes.c_int(0)
+def _decode_workspace(dev: int, *sizes: int) -> int:
     with torch.cuda.device(dev):
-        return int(_lib.get_lib().ab2_kv8_decode_workspace(*sizes, ctypes.addressof(n))), n.value
+        return int(_lib.get_lib().ab2_kv8_decode_workspace(*sizes))
 
 
-_SCRATCH: dict = {}         # (device, stream) -> (counters, workspace) of the calls on that stream
+_SCRATCH: dict = {}         # (device, stream) -> workspace of the calls on that stream
 
 
-def _scratch(dev: int, size: int, n: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """(``n`` counters, a workspace of ``size`` bytes). Calls on one stream run one after the other and share them: every call leaves the
-    counters zero and reads of the workspace only what it has written. A captured call gets its own, the counters cleared in its graph."""
+def _scratch(dev: int, size: int) -> torch.Tensor:
+    """A workspace of ``size`` bytes. Calls on one stream run one after the other and share it: a call reads of it only what it has written. A
+    captured call gets one of its graph's own."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.int32, device=f"cuda:{dev}"), torch.empty(size, dtype=torch.uint8, device=f"cuda:{dev}")
+        return torch.empty(size, dtype=torch.uint8, device=f"cuda:{dev}")
     key = dev, torch._C._cuda_getCurrentRawStream(dev)
     c = _SCRATCH.get(key)
-    if c is None or c[0].numel() < n or c[1].numel() < size:
-        old = (0, 0) if c is None else (c[0].numel(), c[1].numel())
-        c = _SCRATCH[key] = (torch.zeros(max(n, old[0], 1024), dtype=torch.int32, device=f"cuda:{dev}"),
-                             torch.empty(max(size, old[1]), dtype=torch.uint8, device=f"cuda:{dev}"))
+    if c is None or c.numel() < size:
+        c = _SCRATCH[key] = torch.empty(size, dtype=torch.uint8, device=f"cuda:{dev}")
     return c
 
 
@@ -229,9 +225,9 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     ``q`` ``[B, Hq, D]`` bf16, heads dense, rows a multiple of 8 elements apart (the query part of a wider projection); ``Hq`` a multiple of the cache's
     heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous, where given);
     a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
-    length beyond the table, sets the device error word (code 6); the row's result is not to be used. Workspace and
-    counters belong to the current stream or, in a captured call, to its graph: calls on several streams and graphs share neither. At most
-    8192 sequences."""
+    length beyond the table, sets the device error word (code 6); the row's result is not to be used. The workspace
+    belongs to the current stream or, in a captured call, to its graph: calls on several streams and graphs do not share one. At most 8192
+    sequences."""
     shape = q.shape
     if not (len(shape) == 3 and q.dtype is torch.bfloat16):
         raise ValueError("queries: bf16 [B, Hq, D]")
@@ -259,9 +255,9 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
         raise ValueError("heads of a row have to be dense")
     if row & 7 or q.data_ptr() & 15:
         raise ValueError("rows have to start on 16 bytes")
-    counters, ws = _scratch(dev, *_decode_workspace(dev, B, Hq, Hkv, D, ps, width))
+    ws = _scratch(dev, _decode_workspace(dev, B, Hq, Hkv, D, ps, width))
     _launch(dev, "ab2_kv8_decode", q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
-            page_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), counters.data_ptr(), B, Hq, Hkv, D, ps, width, P, scale, row)
+            page_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, Hq, Hkv, D, ps, width, P, scale, row)
     return out
 
 
@@ -342,6 +338,6 @@ def _ints(x) -> list:
 
 
 _lib.declare("ab2_kv8_append", [_V] * 9 + [_I] * 7 + [_L, _L, _V])
-_lib.declare("ab2_kv8_decode", [_V] * 10 + [_I] * 7 + [_F, _L, _V])
-_lib.declare("ab2_kv8_decode_workspace", [_I] * 6 + [_V], _L)
+_lib.declare("ab2_kv8_decode", [_V] * 9 + [_I] * 7 + [_F, _L, _V])
+_lib.declare("ab2_kv8_decode_workspace", [_I] * 6, _L)
 _lib.declare("ab2_copy_pages", [_V, _I, _V, _I, _V])

@@ -210,10 +210,10 @@ kv8_append_page_kernel(const __grid_constant__ Kv8Args a, const int* __restrict_
 // ------------------------------------------------------------------ attention of single tokens
 // o = softmax(scale * q K^T) V over the first lens[b] tokens, G query heads for each key/value head. Bound by the codes' bytes.
 //
-// Split: every (sequence, head) item is cut into units of U chunks of 64 tokens, U from the whole batch's tokens so that a resident wave of
-// blocks gets about KV8_ROUNDS units each, whatever the lengths are. Blocks take units from a counter: SMs do not get equal shares of the
-// memory's rate (the slowest of equal static shares ended 20 % after the mean), so the faster ones take more. The block that
-// finishes the last unit of an item joins its parts. Both kinds of counters wrap to zero with the last count, so they are left as found.
+// Split: every (sequence, head) item is cut into units of U chunks of 64 tokens, U from the whole batch's tokens, whatever the lengths are.
+// Block i takes units i, i + grid, ...: about one each, so that taking them from a counter instead (SMs do not get equal shares of the
+// memory's rate) gained 1 % on the largest case and cost a launch that clears it in every captured call. A second kernel joins the
+// units of items that were split (the last block of an item joining it cost 1.4 us a unit for the fence, which waits for its copies too).
 // Warp w of a block takes tokens 16 w .. 16 w + 15 of each chunk and fetches them itself, with 16-byte asynchronous copies into a ring
 // of its own in shared memory, so there is no barrier in the loop and the bytes in flight are not bounded by registers.
 //   S^T[16 tokens, 8 heads] = K Q^T: the sum over dims may be taken in any order, so 16 contiguous bytes of a row serve a thread as
@@ -224,7 +224,8 @@ kv8_append_page_kernel(const __grid_constant__ Kv8Args a, const int* __restrict_
 // bank conflicts. e4m3 converts to fp16 exactly; q is divided by a power of two for its head (exact), P is rounded to fp16 (11 bits,
 // half a step 2^-12) as e^x scaled so that the largest seen lies between 2^9 and 2^15 (the running maximum only moves when a score leaves
 // that range, so that shares down to 2^-23 of the largest keep all bits), and both sums are fp32.
-constexpr int KV8_CHUNK = 64, KV8_ROUNDS = 1, KV8_MOST_ROWS = 8192;
+constexpr int KV8_CHUNK = 64, KV8_MOST_ROWS = 8192;
+constexpr int KV8_LEAST = 4;        // chunks of the smallest unit: what a split saves of so short an item, the join costs
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -276,7 +277,7 @@ struct Kv8Decode {
   const int *table, *lens;
   __nv_bfloat16* out;
   float *part_o, *part_ml;      // [slots][HP][D], [slots][HP][2]: units of items that are split
-  unsigned int* counters;       // [1 + items], zero: units taken, and units finished of each item
+  int2* meta;                   // [B] units of an item of the sequence, and its first slot
   int* err;
   int B, Hq, Hkv, G, groups, page_size, page_bits, width, num_pages;
   float scale_log2;             // softmax scale * log2(e)
@@ -305,12 +306,13 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
   constexpr int HP = 8 * NT;
   constexpr int KS = D / 16;            // steps of S; also D / 16 row tiles of O
   constexpr int S = Cfg::STAGES;
-  extern __shared__ __align__(128) unsigned char dsm[];       // four rings; where a segment ends, each holds its warp's result [HP][D + 4]
+  extern __shared__ __align__(128) unsigned char dsm[];       // four rings; where a unit ends, each holds its warp's result [HP][D + 4]
   float* mm = reinterpret_cast<float*>(dsm + 4 * Cfg::RING);  // [4][HP]
   float* ml = mm + 4 * HP;                                    // [4][HP]
   int* units = reinterpret_cast<int*>(ml + 4 * HP);           // [B + 1] units of one head before sequence b
   int* slots = units + a.B + 1;                               // [B + 1] those of split items only
-  __shared__ int wsum[2][4], s_next, s_last;
+  __shared__ int wsum[2][4];
+  __shared__ float s_scale[4][S][2];                          // scales of the tiles in the rings
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
@@ -332,7 +334,11 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
   if (lane == 0) wsum[0][warp] = sum;
   __syncthreads();
   const int chunks = (wsum[0][0] + wsum[0][1] + wsum[0][2] + wsum[0][3]) * Hv;
-  const int U = max(1, (int)(((unsigned)chunks + gridDim.x * KV8_ROUNDS - 1) / (gridDim.x * KV8_ROUNDS)));
+  // A unit's chunks: an equal share of the wave. Where the items alone fill half of the wave or more, twice that: a unit costs about 4 us
+  // beside its chunks (queries, first copies, join), and fewer of them cost less than the uneven end does (64 x 1k: 35 us against 39; 12 items of
+  // 32k: 24 us with single shares, 25 with double ones; shares halved or the last quarter cut finer: 2 to 20 % slower in every case).
+  const unsigned share = (unsigned)chunks * (2 * Hv * a.B >= (int)gridDim.x ? 2u : 1u);
+  const int U = max(KV8_LEAST, (int)((share + gridDim.x - 1) / gridDim.x));
   {
     int carry_u = 0, carry_s = 0;
     for (int i0 = 0; i0 < a.B; i0 += 128) {
@@ -357,54 +363,67 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
     if (tid == 0) { units[a.B] = carry_u; slots[a.B] = carry_s; }
     __syncthreads();
   }
+  const int total = units[a.B] * Hv;                            // units
+  for (int i = blockIdx.x * 128 + tid; i < a.B; i += gridDim.x * 128) a.meta[i] = make_int2(units[i + 1] - units[i], slots[i] * Hv);
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)            // rows without tokens
     if (units[b] == units[b + 1])
       for (int i = tid; i < a.Hq * D / 8; i += 128) reinterpret_cast<uint4*>(a.out + (size_t)b * a.Hq * D)[i] = make_uint4(0u, 0u, 0u, 0u);
-  const int total = units[a.B] * Hv;                            // units
-  const int grid = min((int)gridDim.x, total);
 
-  for (int unit = blockIdx.x; unit < total;) {
-    // the next one: every block asks once more than it gets, so there are `total` counts in all
-    unsigned int next = 0;
-    if (tid == 0) next = grid + atomicInc(a.counters, total - 1);
-    // ---- which item, which of its chunks
+  struct Unit { int b, np, hv, part, len, c0, c1; };
+  auto unit_of = [&](int unit) {
     int lo = 0, hi = a.B;                                       // last b with Hv * units[b] <= unit and units of its own
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (units[mid] * Hv <= unit) lo = mid; else hi = mid;
     }
-    const int b = lo, np = units[b + 1] - units[b], rest = unit - units[b] * Hv, hv = rest / np, part = rest - hv * np;
-    const int len = length(b), nc = (len + KV8_CHUNK - 1) / KV8_CHUNK, per = (nc + np - 1) / np;
-    const int c0 = part * per, c1 = min(nc, c0 + per);
+    Unit u;
+    u.b = lo;
+    u.np = units[lo + 1] - units[lo];
+    const int rest = unit - units[lo] * Hv;
+    u.hv = rest / u.np;
+    u.part = rest - u.hv * u.np;
+    u.len = length(lo);
+    const int nc = (u.len + KV8_CHUNK - 1) / KV8_CHUNK, per = (nc + u.np - 1) / u.np;
+    u.c0 = u.part * per;
+    u.c1 = min(nc, u.c0 + per);
+    return u;
+  };
+  // What the next unit is and its pages (lane i: of this warp's tile i) are looked up while this one runs: its first copies then
+  // start at once.
+  Unit u = {};
+  int pg_first = 0;
+  auto tiles_of = [&](const Unit& x) { return min(x.c1 - x.c0, max(0, (x.len - x.c0 * KV8_CHUNK - warp * 16 + KV8_CHUNK - 1) / KV8_CHUNK)); };
+  auto page_of = [&](const Unit& x, int i, int n) {
+    int p = 0;
+    if (i < n) {
+      p = a.table[(size_t)x.b * a.width + (((x.c0 + i) * KV8_CHUNK + warp * 16) >> a.page_bits)];
+      if ((unsigned)p >= (unsigned)a.num_pages) { set_error(a.err, ERR_BOUNDS); p = 0; }
+    }
+    return p;
+  };
+  if ((int)blockIdx.x < total) {
+    u = unit_of(blockIdx.x);
+    pg_first = page_of(u, lane, tiles_of(u));
+  }
+  for (int unit = blockIdx.x; unit < total; unit += gridDim.x) {
+    const int b = u.b, np = u.np, hv = u.hv, part = u.part, len = u.len;
     const int h = hv / a.groups, g0 = (hv - h * a.groups) * 16, ng = min(a.G - g0, HP);
-    const int* pt = a.table + (size_t)b * a.width;
-
-    // ---- this warp's tiles: tokens 64 c + 16 warp of chunks c0 .. c1
-    const int t_first = c0 * KV8_CHUNK + warp * 16;
-    const int n_tiles = min(c1 - c0, max(0, (len - t_first + KV8_CHUNK - 1) / KV8_CHUNK));
-    // Lane i of a block of 32 tiles holds its page (fetched one block ahead), and later its scales (from when its first tile is fetched).
-    int pg = 0, pg_next = 0;
-    float ksc = 0.f, vsc = 0.f, ksc_next = 0.f, vsc_next = 0.f;
-    auto page_of = [&](int i) {
-      int p = 0;
-      if (i < n_tiles) {
-        p = pt[(t_first + i * KV8_CHUNK) >> a.page_bits];
-        if ((unsigned)p >= (unsigned)a.num_pages) { set_error(a.err, ERR_BOUNDS); p = 0; }
-      }
-      return p;
-    };
+    // ---- this warp's tiles: tokens 64 c + 16 warp of the unit's chunks
+    const int t_first = u.c0 * KV8_CHUNK + warp * 16, n_tiles = tiles_of(u);
+    const Unit now = u;
+    int pg = 0, pg_next = pg_first;                             // pages of 32 tiles, and of the next 32
     uint32_t st_in = ring, st_out = ring;                       // stages that the next tile goes to and comes from
+    int sc_in = 0, sc_out = 0;
     auto fetch = [&](int i) {                                   // tile i into its stage; an empty group where there is none
       if (i < n_tiles) {
         if ((i & 31) == 0) {
           pg = pg_next;
-          ksc_next = a.ks[(size_t)pg * a.Hkv + h];
-          vsc_next = a.vs[(size_t)pg * a.Hkv + h];
-          pg_next = page_of(i + 32 + lane);
+          pg_next = n_tiles > i + 32 ? page_of(now, i + 32 + lane, n_tiles) : 0;
         }
-        const int p = __shfl_sync(0xffffffffu, pg, i & 31);
-        const int t = (t_first + i * KV8_CHUNK) & (a.page_size - 1);
-        const size_t at = ((((size_t)p * a.Hkv + h) << a.page_bits) + t) * D + lane * 16;
+        const size_t blk = (size_t)__shfl_sync(0xffffffffu, pg, i & 31) * a.Hkv + h;
+        const size_t at = ((blk << a.page_bits) + ((t_first + i * KV8_CHUNK) & (a.page_size - 1))) * D + lane * 16;
+        if (lane < 2)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&s_scale[warp][sc_in][lane])), "l"((lane ? a.vs : a.ks) + blk) : "memory");
         const unsigned char *ksrc = a.kc + at, *vsrc = a.vc + at;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {                      // 512 bytes of each, contiguous
@@ -414,12 +433,16 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
           copy16_async(d + Cfg::TILE, vsrc + j * 512);
         }
         st_in = st_in == ring + (S - 1) * 2 * Cfg::TILE ? ring : st_in + 2 * Cfg::TILE;
+        sc_in = sc_in == S - 1 ? 0 : sc_in + 1;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    pg_next = page_of(lane);
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) fetch(i);
+    if (unit + (int)gridDim.x < total) {
+      u = unit_of(unit + gridDim.x);
+      pg_first = page_of(u, lane, tiles_of(u));
+    }
 
     // ---- queries as the B operand: head gq of the tile, dims in the order of the keys' bytes
     uint32_t qf[NT][KS][2];
@@ -464,8 +487,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
     float v_last = 0.f;
     uint32_t ratio = 0u;                                        // scale of this page's values over v_ref, as two fp16
     auto work = [&](int i) {
-      if ((i & 31) == 0) { ksc = ksc_next; vsc = vsc_next; }
-      const float kscale = __shfl_sync(0xffffffffu, ksc, i & 31), vscale = __shfl_sync(0xffffffffu, vsc, i & 31);
+      const float kscale = s_scale[warp][sc_out][0], vscale = s_scale[warp][sc_out][1];
+      sc_out = sc_out == S - 1 ? 0 : sc_out + 1;
       const int left = len - (t_first + i * KV8_CHUNK);         // tokens of the tile that exist (16 or more: all)
       const uint32_t kt = st_out, vt = st_out + Cfg::TILE;
       st_out = st_out == ring + (S - 1) * 2 * Cfg::TILE ? ring : st_out + 2 * Cfg::TILE;
@@ -479,15 +502,21 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
         if constexpr (D == 128) *reinterpret_cast<uint4*>(&v[r][0]) = lds16(vt + (v_off ^ ((r & 1) << 4)) + (r & 1) * 128 + (r >> 1) * 1024);
         else *reinterpret_cast<uint2*>(&v[r][0]) = lds8(vt + (v_off ^ ((r & 1) << 6)) + (r >> 1) * 512);
       }
-      float s[NT][4];
+      float s[NT][4], s2[NT][4];                                // two sums of half the dims each: chains half as long
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = s2[t][e] = 0.f;
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
         const uint32_t a0 = half2_lo(k[0][j]), a2 = half2_hi(k[0][j]), a1 = half2_lo(k[1][j]), a3 = half2_hi(k[1][j]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma_f16_16816(s[t], a0, a1, a2, a3, qf[t][j][0], qf[t][j][1]);
+        for (int t = 0; t < NT; ++t) mma_f16_16816(j & 1 ? s2[t] : s[t], a0, a1, a2, a3, qf[t][j][0], qf[t][j][1]);
       }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] += s2[t][e];
       if (left < 16) {                                          // what stands behind the last token may be anything
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -615,57 +644,64 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)slot * HP + g) * 2) = make_float2(mx, l);
       }
     }
-    if (np > 1) {
-      // ---- the item's last unit joins them: a warp for each head, lane i weighs part i, all lanes read its row together
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        s_last = atomicInc(a.counters + 1 + b * Hv + hv, np - 1) == (unsigned)(np - 1);
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        const size_t first = (size_t)(slot - part) * HP;
-        constexpr int PER = D / 32;
-        for (int g = warp; g < ng; g += 4) {
-          float mx = -INFINITY, l = 0.f, acc[PER];
+    __syncthreads();                                            // the rings are free for the next unit
+  }
+}
+
+// Joins the units of split items. Block (b, y) takes the heads y, y + gridDim.y, ... of sequence b: four warps share an item's units, lane i
+// weighs unit i, all lanes read its row together, eight rows on their way at a time.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ Kv8Decode a) {
+  constexpr int HP = 8 * NT, PER = D / 32;
+  __shared__ float so[4][D], sm[4], sl[4];
+  pdl_wait();
+  pdl_trigger();
+  const int2 meta = a.meta[blockIdx.x];
+  const int b = blockIdx.x, np = meta.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (np <= 1) return;
+  for (int hq = blockIdx.y; hq < a.Hq; hq += gridDim.y) {
+    const int h = hq / a.G, gh = hq - h * a.G, grp = gh / 16, g = gh - grp * 16;
+    const size_t first = (size_t)(meta.y + (h * a.groups + grp) * np);
+    float mx = -INFINITY, l = 0.f, acc[PER];
 #pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-          for (int i0 = 0; i0 < np; i0 += 32) {
-            const float2 p = i0 + lane < np ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + (first + (size_t)(i0 + lane) * HP + g) * 2)) : make_float2(-INFINITY, 0.f);
-            const float m = fmaxf(mx, warp_max(p.x)), f0 = fast_exp2(mx - m), f = fast_exp2(p.x - m);
-            mx = m;
-            l = l * f0 + p.y * f;
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    for (int i0 = warp; i0 < np; i0 += 128) {                   // units i0, i0 + 4, ...: 32 of them
+      const int i = i0 + 4 * lane, n = min(32, (np - i0 + 3) / 4);
+      const float2 p = i < np ? *reinterpret_cast<const float2*>(a.part_ml + ((first + i) * HP + g) * 2) : make_float2(-INFINITY, 0.f);
+      const float m = fmaxf(mx, warp_max(p.x)), f0 = fast_exp2(mx - m), f = fast_exp2(p.x - m);
+      mx = m;
+      l = l * f0 + p.y * f;
 #pragma unroll
-            for (int e = 0; e < PER; ++e) acc[e] *= f0;
-            const float* src = a.part_o + (first + (size_t)i0 * HP + g) * D + lane * PER;
-            const int n = min(32, np - i0);
-            for (int i = 0; i < n; i += 8) {                    // eight rows on their way at a time
-              float x[8][PER];
+      for (int e = 0; e < PER; ++e) acc[e] *= f0;
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        float x[8][PER];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float* p = src + (size_t)min(i + j, n - 1) * HP * D;
-                if constexpr (D == 128) *reinterpret_cast<float4*>(x[j]) = __ldcg(reinterpret_cast<const float4*>(p));
-                else *reinterpret_cast<float2*>(x[j]) = __ldcg(reinterpret_cast<const float2*>(p));
-              }
+        for (int j = 0; j < 8; ++j) {
+          const float* q = a.part_o + ((first + i0 + 4 * min(j0 + j, n - 1)) * HP + g) * D + lane * PER;
+          if constexpr (D == 128) *reinterpret_cast<float4*>(x[j]) = *reinterpret_cast<const float4*>(q);
+          else *reinterpret_cast<float2*>(x[j]) = *reinterpret_cast<const float2*>(q);
+        }
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float w = __shfl_sync(0xffffffffu, f, i + j);            // lanes behind the last part hold zero
+        for (int j = 0; j < 8; ++j) {
+          const float w = __shfl_sync(0xffffffffu, f, j0 + j);  // lanes behind the last unit hold zero
 #pragma unroll
-                for (int e = 0; e < PER; ++e) acc[e] += x[j][e] * w;
-              }
-            }
-          }
-          const float inv = 1.f / warp_sum(l);
-          uint32_t* out = reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.Hq + h * a.G + g0 + g) * D + lane * PER);
-#pragma unroll
-          for (int e = 0; e < PER / 2; ++e) out[e] = pack_bf16(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+          for (int e = 0; e < PER; ++e) acc[e] += x[j][e] * w;
         }
       }
     }
-    if (tid == 0) s_next = (int)next;
-    __syncthreads();                                            // the buffers are free for the next unit
-    unit = s_next;
+    l = warp_sum(l);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) so[warp][lane * PER + e] = acc[e];
+    if (lane == 0) { sm[warp] = mx; sl[warp] = l; }
+    __syncthreads();
+    mx = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    l = 0.f;
+    float f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { f[w] = fast_exp2(sm[w] - mx); l += sl[w] * f[w]; }
+    for (int d = threadIdx.x; d < D; d += 128)
+      a.out[((size_t)b * a.Hq + hq) * D + d] = __float2bfloat16((so[0][d] * f[0] + so[1][d] * f[1] + so[2][d] * f[2] + so[3][d] * f[3]) / l);
+    __syncthreads();
   }
 }
 
@@ -677,6 +713,11 @@ static int launch_kv8_decode(const Kv8Decode& a, int grid, cudaStream_t s) {
   static ab2host::DevState st;
   if (ab2host::prepare_launch(kern, RING + 2 * (KV8_MOST_ROWS + 1) * 4, st, nullptr)) return 2;
   launch_pdl(kern, dim3(grid), dim3(128), (size_t)smem, s, a);
+  if (((long long)a.width * a.page_size + KV8_CHUNK - 1) / KV8_CHUNK > KV8_LEAST) {              // some item may have been split
+    int y = 4736 / a.B;
+    y = y < 1 ? 1 : y > a.Hq ? a.Hq : y;
+    launch_pdl(kv8_join_kernel<D, NT>, dim3(a.B, y), dim3(128), 0, s, a);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : 1;
 }
 
@@ -790,20 +831,18 @@ static int kv8_grid(int B, int Hq, int Hkv, int width, int page_size, int sms) {
   const long long wave = (long long)sms * (G <= 8 ? Kv8Cfg<128, 1>::BLOCKS : Kv8Cfg<128, 2>::BLOCKS);
   return (int)(most < wave ? most : wave);
 }
-// Bytes of the workspace, and in *counters the unsigned counters beside it. A split item has at least two units, so no more than
-// 2 * blocks * rounds units belong to split items.
-long long ab2_kv8_decode_workspace(int B, int Hq, int Hkv, int D, int page_size, int width, int* counters) {
+// Bytes of the workspace. A split item has at least two units, and a unit is a block's share or more, so no more than 2 * blocks units belong to split items.
+long long ab2_kv8_decode_workspace(int B, int Hq, int Hkv, int D, int page_size, int width) {
   if (B <= 0 || Hkv <= 0 || Hq % Hkv) return 0;
-  const int G = Hq / Hkv, groups = (G + 15) / 16, HP = G <= 8 ? 8 : 16;
-  *counters = 1 + B * Hkv * groups;
-  const long long slots = 2LL * KV8_ROUNDS * kv8_grid(B, Hq, Hkv, width, page_size, ab2_num_sms());
-  return slots * HP * (D + 2) * 4;
+  const int G = Hq / Hkv, HP = G <= 8 ? 8 : 16;
+  const long long slots = 2LL * kv8_grid(B, Hq, Hkv, width, page_size, ab2_num_sms());
+  return slots * HP * (D + 2) * 4 + (long long)B * 8;
 }
 
-// q [B, Hq, D] bf16 (rows q_stride elements apart, heads dense), out [B, Hq, D] dense; cache and table as above; lens [B]. The counters are
-// zero before the call and after it; calls that may run at the same time must not share them or the workspace.
+// q [B, Hq, D] bf16 (rows q_stride elements apart, heads dense), out [B, Hq, D] dense; cache and table as above; lens [B]. Calls that
+// may run at the same time must not share the workspace.
 int ab2_kv8_decode(const void* q, const void* kc, const void* vc, const void* ks, const void* vs, const int* table, const int* lens, void* out,
-                   void* workspace, void* counters, int B, int Hq, int Hkv, int D, int page_size, int width, int num_pages, float scale, long long q_stride,
+                   void* workspace, int B, int Hq, int Hkv, int D, int page_size, int width, int num_pages, float scale, long long q_stride,
                    void* stream) {
   if (B <= 0) return 0;
   if (D != 64 && D != 128) return 11;
@@ -821,8 +860,8 @@ int ab2_kv8_decode(const void* q, const void* kc, const void* vc, const void* ks
   a.scale_log2 = scale * 1.4426950408889634f; a.q_stride = q_stride; a.err = ab2host::error_flag();
   const int HP = G <= 8 ? 8 : 16;
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + 2LL * KV8_ROUNDS * grid * HP * D;
-  a.counters = (unsigned int*)counters;
+  a.part_ml = a.part_o + 2LL * grid * HP * D;
+  a.meta = (int2*)(a.part_ml + 2LL * grid * HP * 2);
   cudaStream_t s = (cudaStream_t)stream;
   if (D == 128) return G <= 8 ? launch_kv8_decode<128, 1>(a, grid, s) : launch_kv8_decode<128, 2>(a, grid, s);
   return G <= 8 ? launch_kv8_decode<64, 1>(a, grid, s) : launch_kv8_decode<64, 2>(a, grid, s);

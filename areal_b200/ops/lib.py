@@ -124,7 +124,7 @@ def get_lib():
 
 
 # Number of kernels each exported launcher enqueues (used for launch accounting).
-_KERNELS_PER_CALL = {"ab2_kernel_error_peek": 0, "ab2_gemm_splitk": 2, "ab2_paged_decode": 2, "ab2_paged_decode_strided": 2, "ab2_paged_decode_noalloc": 2, "ab2_kv8_decode_workspace": 0, "ab2_kernel_error": 0, "ab2_runtime_init": 0, "ab2_num_sms": 0}
+_KERNELS_PER_CALL = {"ab2_kernel_error_peek": 0, "ab2_gemm_splitk": 2, "ab2_paged_decode": 2, "ab2_paged_decode_strided": 2, "ab2_paged_decode_noalloc": 2, "ab2_kv8_decode": 2, "ab2_kv8_decode_workspace": 0, "ab2_kernel_error": 0, "ab2_runtime_init": 0, "ab2_num_sms": 0}
 LAUNCHES = {"count": 0}
 
 
