@@ -19,8 +19,10 @@ import sys
 
 import torch
 
+from . import cache_ops as CO
 from . import functional as OF
 from . import lib as oplib
+from . import sampling as SO
 
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
@@ -232,6 +234,53 @@ def bench_decode(a):
     return report("paged_decode_attention", ms, 0.0, by, batch=a.batch, ctx=a.ctx)
 
 
+def _kv8_case(a, lens):
+    """(pages, page table, lengths) of an 8-bit cache with ``lens`` tokens for each of the batch's rows."""
+    ps = 64
+    width = max(lens) // ps + 1
+    n = a.batch * width
+    x = torch.randn(n, a.kv_heads, ps, a.dim, device="cuda")
+    p = CO.QuantPages.empty(n, a.kv_heads, ps, a.dim, "cuda")
+    for c, s in ((p.k, p.k_scale), (p.v, p.v_scale)):
+        c.copy_((x * 64).to(CO.F8))
+        s.fill_(2.0 ** -6)
+    return p, torch.randperm(n, device="cuda").int().view(a.batch, width).contiguous(), torch.tensor(lens, device="cuda", dtype=torch.int32)
+
+
+def bench_kv8_decode(a):
+    p, table, lens = _kv8_case(a, [a.ctx] * a.batch)
+    q = torch.randn(a.batch, a.heads, a.dim, device="cuda").bfloat16()
+    ms = timeit(lambda: CO.kv8_decode(q, p, table, lens), a.iters, a.warmup)
+    return report("kv8_decode_attention", ms, 4.0 * a.batch * a.ctx * a.heads * a.dim, 2.0 * a.batch * a.ctx * a.kv_heads * a.dim, batch=a.batch, ctx=a.ctx)
+
+
+def bench_kv8_append(a):
+    p, table, lens = _kv8_case(a, [a.ctx] * a.batch)
+    T = a.batch * a.ctx
+    k, v = (torch.randn(T, a.kv_heads, a.dim, device="cuda").bfloat16() for _ in range(2))
+    cu = torch.arange(a.batch + 1, device="cuda", dtype=torch.int32) * a.ctx
+    ms = timeit(lambda: CO.kv8_append(k, v, p, table, lens, cu), a.iters, a.warmup)
+    return report("kv8_append", ms, 0.0, 3.0 * 2 * T * a.kv_heads * a.dim, tokens=T)
+
+
+def bench_copy_pages(a):
+    """``batch`` pages of a cache of ``layers`` layers (28 where not given), 16 bits."""
+    L, n = a.layers or 28, a.batch
+    d = torch.randn(L, 2, 2 * n, 64, a.kv_heads, a.dim, device="cuda").bfloat16()
+    ms = timeit(lambda: CO.copy_pages([(d, 2, 3)], list(range(n)), list(range(n, 2 * n))), a.iters, a.warmup)
+    return report("copy_pages", ms, 0.0, 2.0 * d.numel(), pages=n, layers=L)
+
+
+def bench_sample_filtered(a):
+    """``batch`` rows, top-p 0.95, a few tokens far above the others as in a trained model's logits."""
+    x = torch.randn(a.batch, a.vocab, device="cuda") * 2.3
+    x.scatter_add_(1, torch.randint(0, a.vocab, (a.batch, 40), device="cuda"), torch.rand(a.batch, 40, device="cuda") * 16)
+    one, u = torch.ones(a.batch, device="cuda"), torch.rand(a.batch, device="cuda")
+    k = torch.zeros(a.batch, device="cuda", dtype=torch.int32)
+    ms = timeit(lambda: SO.sample_filtered(x, u, one, k, one * 0.95, one * 0), a.iters, a.warmup)
+    return report("sample_filtered", ms, 0.0, 4.0 * a.batch * a.vocab, rows=a.batch, vocab=a.vocab)
+
+
 def bench_rmsnorm(a):
     x = torch.randn(a.rows, a.hidden, device="cuda").bfloat16()
     r = torch.randn_like(x)
@@ -399,7 +448,7 @@ def bench_push_plan(a):
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["gemm", "gemm_decode", "gemm_fp8", "gemm_skinny", "qknorm_rope", "attn_fwd", "attn_bwd", "decode", "rmsnorm", "swiglu", "adamw", "logprob",
+    ap.add_argument("kernel", choices=["gemm", "gemm_decode", "gemm_fp8", "gemm_skinny", "qknorm_rope", "attn_fwd", "attn_bwd", "decode", "kv8_decode", "kv8_append", "copy_pages", "sample_filtered", "rmsnorm", "swiglu", "adamw", "logprob",
                                            "engine_decode", "ep", "push_plan", "moe_route"])
     ap.add_argument("--experts", type=int, default=128); ap.add_argument("--topk", type=int, default=8)
     ap.add_argument("--shards", type=int, default=4); ap.add_argument("--tp", type=int, default=2); ap.add_argument("--replicas", type=int, default=2)
@@ -419,7 +468,8 @@ def main(argv=None):
     a = ap.parse_args(argv)
     if a.kernel == "logprob" and a.rows > 4096:
         a.rows = 2048
-    return {"gemm": bench_gemm, "gemm_decode": bench_gemm_decode, "gemm_fp8": bench_gemm_fp8, "gemm_skinny": bench_gemm_skinny, "qknorm_rope": bench_qknorm_rope, "attn_fwd": bench_attn_fwd, "attn_bwd": bench_attn_bwd, "decode": bench_decode,
+    return {"gemm": bench_gemm, "gemm_decode": bench_gemm_decode, "gemm_fp8": bench_gemm_fp8, "gemm_skinny": bench_gemm_skinny, "qknorm_rope": bench_qknorm_rope, "attn_fwd": bench_attn_fwd, "attn_bwd": bench_attn_bwd, "decode": bench_decode, "kv8_decode": bench_kv8_decode, "kv8_append": bench_kv8_append, "copy_pages": bench_copy_pages,
+            "sample_filtered": bench_sample_filtered,
             "rmsnorm": bench_rmsnorm, "swiglu": bench_swiglu, "adamw": bench_adamw, "logprob": bench_logprob,
             "engine_decode": bench_engine_decode, "ep": bench_ep, "push_plan": bench_push_plan, "moe_route": bench_moe_route}[a.kernel](a)
 
