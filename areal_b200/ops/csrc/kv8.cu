@@ -740,6 +740,10 @@ struct CopyArgs {
 template <typename T>
 __device__ __forceinline__ void copy_run(const unsigned char* s, unsigned char* d, int run, long long row_stride, int first, int last) {
   constexpr int U = sizeof(T), PER = COPY_PER;
+  // the row of access i without an integer division for each: counted from the block's first row, where a quotient in single precision is
+  // off by one at most
+  const int len = run / U, row0 = first / run, base = row0 * len;
+  const float inv = 1.f / (float)len;
   for (int i0 = first / U + threadIdx.x; i0 < last / U; i0 += PER * 256) {
     T v[PER];
     long long off[PER];
@@ -747,8 +751,10 @@ __device__ __forceinline__ void copy_run(const unsigned char* s, unsigned char* 
     for (int j = 0; j < PER; ++j) {
       const int i = i0 + j * 256;
       if (i < last / U) {
-        const int row = i / (run / U);
-        off[j] = row * row_stride + (long long)(i - row * (run / U)) * U;
+        int q = (int)((float)(i - base) * inv), rest = i - base - q * len;
+        if (rest < 0) { --q; rest += len; }
+        if (rest >= len) { ++q; rest -= len; }
+        off[j] = (row0 + q) * row_stride + (long long)rest * U;
         v[j] = *reinterpret_cast<const T*>(s + off[j]);
       }
     }

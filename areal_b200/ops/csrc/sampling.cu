@@ -38,6 +38,7 @@ constexpr int SF_CAP = 2048;           // entries of the list
 constexpr int SF_SEG = 256;            // logits of a piece of a block's share that has a sum of its own
 constexpr int SF_SEGS = 200;           // at most
 constexpr float SF_FAR = 16.6f;        // nats below the maximum from where single precision will do for a total (2^-24 of the maximum)
+constexpr int SF_LOADS = 10;           // 16-byte loads of a thread on their way: a share of 20480 logits at once
 constexpr int SF_GUESS = 256;          // tokens of a nucleus that is tried without a histogram of the row
 constexpr int SF_MAX_CLUSTER = 8;
 constexpr float SF_PER_NAT = 64.f;
@@ -279,15 +280,19 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   float mx = -INFINITY;
   {
     const float* src = a.logits + (size_t)row * a.ld + begin;
-    auto clean = [](float x) { return x == x ? x : -INFINITY; };
+    auto clean = [](float x) { return fmaxf(x, -INFINITY); };               // NaN has no weight
     if (a.aligned) {
       const int n4 = n >> 2;
-#pragma unroll 4
-      for (int i = tid; i < n4; i += SF_THREADS) {
-        float4 v = __ldcs(reinterpret_cast<const float4*>(src) + i);
-        v.x = clean(v.x); v.y = clean(v.y); v.z = clean(v.z); v.w = clean(v.w);
-        reinterpret_cast<float4*>(xs)[i] = v;
-        mx = fmaxf(mx, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+      for (int i0 = tid; i0 < n4; i0 += SF_LOADS * SF_THREADS) {                        float4 v[SF_LOADS];
+#pragma unroll
+        for (int j = 0; j < SF_LOADS; ++j)
+          v[j] = i0 + j * SF_THREADS < n4 ? __ldcs(reinterpret_cast<const float4*>(src) + i0 + j * SF_THREADS) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll
+        for (int j = 0; j < SF_LOADS; ++j) {
+          v[j].x = clean(v[j].x); v[j].y = clean(v[j].y); v[j].z = clean(v[j].z); v[j].w = clean(v[j].w);
+          if (i0 + j * SF_THREADS < n4) reinterpret_cast<float4*>(xs)[i0 + j * SF_THREADS] = v[j];
+          mx = fmaxf(mx, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+        }
       }
       for (int i = 4 * n4 + tid; i < n; i += SF_THREADS) { const float v = clean(src[i]); xs[i] = v; mx = fmaxf(mx, v); }
     } else {
@@ -357,10 +362,17 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   if (greedy) {
     double s = 0.0;
     int first = 0x7fffffff;
-    for (int i = tid; i < n; i += SF_THREADS) {
-      const float x = xs[i];
-      s += w_of(x);
-      if (x == xmax) first = min(first, begin + i);
+#pragma unroll 2
+    for (int i = tid; i < a.share / 4; i += SF_THREADS) {
+      const float4 v = reinterpret_cast<const float4*>(xs)[i];
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      double w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = weight(fma((double)x[j], it, -top_it), sh.tab);
+        if (x[j] == xmax) { first = min(first, begin + 4 * i + j); w[j] = 1.0; }
+      }
+      s += (w[0] + w[1]) + (w[2] + w[3]);
     }
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) sh.ired[warp] = first;
