@@ -60,7 +60,7 @@ def _check_pages(p: QuantPages, dim: int, dev: int) -> tuple:
     if (len(s) == 4 and v.shape == s and k.dtype is F8 and v.dtype is F8 and ks.dtype is torch.float32 and vs.dtype is torch.float32 and ks.shape == s[:2]
             and vs.shape == s[:2] and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and s[2] in PAGE_SIZES
             and s[3] == dim and (dim == 128 or dim == 64) and s[0] > 0 and s[1] > 0
-            and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == dev):
+            and k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == dev and not (k.data_ptr() | v.data_ptr()) & 15):
         return s[0], s[1], s[2]
     # which of them it is
     _need(k.dtype == F8 and v.dtype == F8 and len(s) == 4 and v.shape == s, "codes: two e4m3 tensors [pages, Hkv, page_size, D]")
@@ -70,6 +70,7 @@ def _check_pages(p: QuantPages, dim: int, dev: int) -> tuple:
     _need(s[3] == dim and dim in (64, 128), f"head size {dim} with a cache of {s[3]}: 64 or 128 are built")
     _need(s[2] in PAGE_SIZES, f"page size {s[2]}: one of {PAGE_SIZES}")
     _need(s[0] > 0 and s[1] > 0, "a cache without pages or heads")
+    _need(not (k.data_ptr() | v.data_ptr()) & 15, "codes have to start on 16 bytes")
     raise ValueError("cache on another device than the rows")
 
 
@@ -223,8 +224,8 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     """Attention of one query token per sequence over its first ``seq_lens[b]`` cached tokens: ``softmax(scale q K^T) V``.
 
     ``q`` ``[B, Hq, D]`` bf16, heads dense, rows a multiple of 8 elements apart (the query part of a wider projection); ``Hq`` a multiple of the cache's
-    heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous, where given);
-    a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
+    heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous and apart from
+    ``q``, where given); a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
     length beyond the table, sets the device error word (code 6); the row's result is not to be used. The workspace
     belongs to the current stream or, in a captured call, to its graph: calls on several streams and graphs do not share one. At most 8192
     sequences."""
@@ -240,6 +241,10 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
         raise ValueError("more than 8192 sequences, or a table wider than 2^31 tokens")
     if out is not None:
         _need(out.shape == shape and out.dtype == torch.bfloat16 and out.is_contiguous() and out.get_device() == dev, "out: contiguous bf16 like the queries")
+        o, first = out.data_ptr(), q.data_ptr()
+        _need(not o & 15, "out has to start on 16 bytes")
+        _need(not out.numel() or o + 2 * out.numel() <= first or first + 2 * (1 + sum((n - 1) * st for n, st in zip(shape, q.stride()))) <= o,
+              "out overlaps the queries, which other blocks may still read")
     if scale is None:
         scale = D ** -0.5
     if dev < 0:

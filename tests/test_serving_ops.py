@@ -137,6 +137,41 @@ def test_decode_refuses(what):
         CO.kv8_decode(q, p, table, lens, **kw)
 
 
+def _off(shape, dtype, by):
+    """Contiguous zeros that start ``by`` bytes behind an allocation's beginning."""
+    n = int(np.prod(shape)) * torch.empty(0, dtype=dtype).element_size()
+    return torch.zeros(n + 16, dtype=torch.uint8)[by:by + n].view(dtype).view(shape)
+
+
+@pytest.mark.parametrize("what", ["k", "v", "out"])
+def test_what_is_read_or_written_sixteen_bytes_at_a_time_has_to_start_there(what):
+    a = _append_args()
+    q, kw = torch.zeros(3, 4, 64, dtype=torch.bfloat16), {}
+    if what == "out":
+        kw["out"] = _off(q.shape, q.dtype, 2)
+    else:
+        setattr(a[2], what, _off(a[2].k.shape, F8, 8))
+        with pytest.raises(ValueError, match="16 bytes"):
+            CO.kv8_append(*a)
+    with pytest.raises(ValueError, match="16 bytes"):
+        CO.kv8_decode(q, *a[2:], **kw)
+
+
+@pytest.mark.parametrize("shift,fits", [(0, False), (64, False), (9 * 64, False), (10 * 64, True)])
+def test_decode_refuses_an_output_over_its_queries(shift, fits):
+    """Queries are heads 0 to 3 of rows of 6, 2 rows: they end behind 10 heads."""
+    a = _append_args()
+    buf = torch.zeros(40 * 64, dtype=torch.bfloat16)
+    q = buf[:12 * 64].view(2, 6, 64)[:, :4]
+    out = buf[shift:][:8 * 64].view(2, 4, 64)
+    args = (q, a[2], a[3][:2].contiguous(), a[4][:2].contiguous())
+    if fits:
+        assert CO.kv8_decode(*args, out=out) is out
+    else:
+        with pytest.raises(ValueError, match="overlaps"):
+            CO.kv8_decode(*args, out=out)
+
+
 @pytest.mark.parametrize("src,dst,tokens", [([1], [1], None), ([0, 1], [2, 2], None), ([0, 2], [2, 3], None), ([0], [6], None), ([-1], [2], None), ([0], [1, 2], None),
                                             ([0], [1], [17]), ([0], [1], [-1]), ([0, 1], [2, 3], [4])])
 def test_copies_refuse(src, dst, tokens):
