@@ -214,6 +214,8 @@ class NativeInferenceEngine(InferenceEngine):
         self._ragged = bool(getattr(self.model_config, "is_mixer_stack", False))
         if getattr(self.model_config, "learned_positions", False):
             self._context_limit = min(self._context_limit, self.model_config.max_position_embeddings)
+        if self.icfg.kv_cache_dtype in EIGHT_BIT_CACHES and (self._ragged or self._recompute_decode or self.device.type != "cuda"):
+            logger.warning("kv_cache_dtype %r belongs to the paged cache of decoders on CUDA: this engine keeps its states in the model's type", self.icfg.kv_cache_dtype)
         if self._ragged:
             self._init_ragged()
         elif self.device.type == "cuda" and not self._recompute_decode:

@@ -56,6 +56,15 @@ def test_unknown_sampling_places_are_refused():
         NativeInferenceEngine(InferenceEngineConfig(), NativeInferConfig(filtered_sampling="gpu"), model_config=preset("tiny-qwen3"))
 
 
+def test_an_eight_bit_cache_that_cannot_be_had_is_said(monkeypatch):
+    said = []
+    monkeypatch.setattr(IE.logger, "warning", lambda text, *a: said.append(text % a))
+    model = build_model(preset("tiny-qwen3"), dtype=torch.float32, device="cpu", seed=3)
+    for kind, n in (("bfloat16", 0), ("fp8_e4m3", 1)):
+        _engine(model, "cpu", kv_cache_dtype=kind).destroy()
+        assert len([x for x in said if "kv_cache_dtype" in x]) == n
+
+
 def test_an_eight_bit_pool_holds_nearly_twice_the_pages():
     cfg = preset("qwen3-8b")
     a, b = PagedKVCache.bytes_per_page(cfg, 64), PagedKVCache.bytes_per_page(cfg, 64, True)
