@@ -480,7 +480,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int i = 0; i < KS; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
-      m_run[t][0] = m_run[t][1] = -1e30f;
+      m_run[t][0] = m_run[t][1] = -3e38f;                       // below every finite score, and a difference of two such is no NaN
       l_run[t][0] = l_run[t][1] = 0.f;
     }
 
@@ -524,7 +524,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) v[r][c] = 0u;
       }
-      // x = score - running maximum; both of a head's tokens
+      // x = score - running maximum; both of a head's tokens. The product is rounded as the maximum's was: with one rounding for both steps, large
+      // scores (2^24 and more) would be off by the rounding of the maximum's product, whole powers of two.
       float x[NT][4], f[NT][2];
       bool grow = false;
 #pragma unroll
@@ -532,7 +533,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           f[t][e & 1] = qs[t][e & 1] * kscale;
-          x[t][e] = fmaf(s[t][e], f[t][e & 1], -m_run[t][e & 1]);
+          x[t][e] = __fmul_rn(s[t][e], f[t][e & 1]) - m_run[t][e & 1];
         }
         if (left < 16) {
           if (gq >= left) x[t][0] = x[t][1] = -INFINITY;
@@ -548,15 +549,15 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
             // from the products: the old maximum may be so far off that the difference has lost its low bits. Every lane takes
             // part in the exchange; which heads move is the same for the eight lanes of a head only.
             const bool in0 = gq < left, in1 = gq + 8 < left;
-            float top = fmaxf(in0 ? s[t][e] * f[t][e] : -INFINITY, in1 ? s[t][e + 2] * f[t][e] : -INFINITY);
+            float top = fmaxf(in0 ? __fmul_rn(s[t][e], f[t][e]) : -INFINITY, in1 ? __fmul_rn(s[t][e + 2], f[t][e]) : -INFINITY);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - 9.f;              // the largest becomes 2^9
             if (top > m_run[t][e]) {
               const float al = fast_exp2(m_run[t][e] - top);
               m_run[t][e] = top;
-              x[t][e] = in0 ? fmaf(s[t][e], f[t][e], -top) : -INFINITY;
-              x[t][e + 2] = in1 ? fmaf(s[t][e + 2], f[t][e], -top) : -INFINITY;
+              x[t][e] = in0 ? __fmul_rn(s[t][e], f[t][e]) - top : -INFINITY;
+              x[t][e + 2] = in1 ? __fmul_rn(s[t][e + 2], f[t][e]) - top : -INFINITY;
               l_run[t][e] *= al;
 #pragma unroll
               for (int i2 = 0; i2 < KS; ++i2) { o[t][i2][e] *= al; o[t][i2][e + 2] *= al; }

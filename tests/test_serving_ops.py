@@ -382,6 +382,24 @@ def test_decode_values_out_of_the_ordinary():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("exponent", [-20, -8, 0, 60])
+def test_decode_of_large_equal_scores(exponent, sign):
+    """Equal keys, scores of 2^44 (2^37 * 128 dims) times 2^exponent: the mean of the values. As the scores are equal to the last bit, they add nothing to
+    the bound."""
+    for lens in ([40], [700], [3, 0, 2000]):
+        q, p, table, n = _decode_case(len(lens), 8, 2, 128, 16, lens, 12)
+        q.fill_(sign * 2.0 ** 37)
+        p.k.view(torch.uint8)[:] = torch.ones(1).to(F8).view(torch.uint8)
+        p.k_scale.fill_(2.0 ** exponent)
+        q0 = q * 0
+        ref = CO.kv8_decode_ref(q, p, table, n, 1.0)
+        out = CO.kv8_decode(q.cuda(), _clone(p, "cuda"), table.cuda(), n.cuda(), 1.0).cpu()
+        _no_kernel_error()
+        assert torch.all((out.double() - ref).abs() <= _decode_bound(q0, p, table, n, 1.0, ref))
+
+
+@pytest.mark.gpu
 def test_decode_takes_parts_of_a_projection_and_reports_bad_tables():
     q, p, table, n = _decode_case(5, 8, 2, 64, 32, [40, 1, 200, 0, 64], 4)
     z = torch.randn(5, 12 * 64).bfloat16().cuda()
