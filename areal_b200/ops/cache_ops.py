@@ -227,8 +227,8 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous and apart from
     ``q``, where given); a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
     length beyond the table, sets the device error word (code 6); the row's result is not to be used. The workspace
-    belongs to the current stream or, in a captured call, to its graph: calls on several streams and graphs do not share one. At most 8192
-    sequences."""
+    belongs to the current stream or, in a captured call, to its graph: calls on several streams and graphs do not share one, and calls of several threads on
+    one stream go one after the other. At most 8192 sequences."""
     shape = q.shape
     if not (len(shape) == 3 and q.dtype is torch.bfloat16):
         raise ValueError("queries: bf16 [B, Hq, D]")
@@ -250,6 +250,9 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     if dev < 0:
         o = kv8_decode_ref(q, pages, page_table, seq_lens, scale).to(torch.bfloat16)
         return o if out is None else out.copy_(o)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):                 # whose stream it is that may be captured, and that the workspace belongs to
+            return kv8_decode(q, pages, page_table, seq_lens, scale, out)
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
     if B == 0:
@@ -285,7 +288,7 @@ def copy_pages(buffers: Sequence[tuple], src, dst, tokens=None) -> None:
     ``buffers``: up to four ``(tensor, page_dim, token_dim)``. The tensor is contiguous; its dims before ``page_dim`` (layers, keys and values) are copied
     for every page; ``token_dim`` (behind ``page_dim``) counts the tokens of a page, or is None for what belongs to a page as a whole (scales).
     ``src``, ``dst``, ``tokens``: host sequences of ints or integer arrays; ``tokens[i]`` leading tokens of page i are copied, the rest of the
-    destination stays as it is (None: whole pages). A source may stand for several destinations; no page may be a destination twice, or source and
+    destination stays as it is (None: whole pages). They are arguments of the launch: a captured call copies the same pages in every replay. A source may stand for several destinations; no page may be a destination twice, or source and
     destination at once."""
     src, dst = _ints(src), _ints(dst)
     n = len(src)

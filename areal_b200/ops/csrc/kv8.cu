@@ -5,6 +5,8 @@
 // quantising rounds once, and a block whose scale has to grow (a larger row arrives) is re-coded without a second rounding
 // except where a code falls below e4m3's normal range. e4m3 is a floating format, so a scale that is not a power of two would
 // not make its relative steps any finer.
+#include <mutex>
+
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -706,6 +708,9 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ K
   }
 }
 
+// Host threads that share a stream share its workspace: one call's two launches must not have another's between them.
+static std::mutex g_kv8_pair;
+
 template <int D, int NT>
 static int launch_kv8_decode(const Kv8Decode& a, int grid, cudaStream_t s) {
   constexpr int HP = 8 * NT, RING = 4 * Kv8Cfg<D, NT>::RING + 8 * HP * 4;
@@ -713,6 +718,7 @@ static int launch_kv8_decode(const Kv8Decode& a, int grid, cudaStream_t s) {
   auto kern = kv8_decode_kernel<D, NT>;
   static ab2host::DevState st;
   if (ab2host::prepare_launch(kern, RING + 2 * (KV8_MOST_ROWS + 1) * 4, st, nullptr)) return 2;
+  std::lock_guard<std::mutex> lk(g_kv8_pair);
   launch_pdl(kern, dim3(grid), dim3(128), (size_t)smem, s, a);
   if (((long long)a.width * a.page_size + KV8_CHUNK - 1) / KV8_CHUNK > KV8_LEAST) {              // some item may have been split
     int y = 4736 / a.B;

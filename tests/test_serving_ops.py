@@ -1,6 +1,7 @@
 """The 8-bit paged cache (append, attention of single tokens), page copies and filtered sampling, against plain statements in
 64 bits. What runs without a GPU checks the statements themselves and every refusal."""
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -385,11 +386,12 @@ def test_decode_values_out_of_the_ordinary():
 @pytest.mark.parametrize("sign", [-1.0, 1.0])
 @pytest.mark.parametrize("exponent", [-20, -8, 0, 60])
 def test_decode_of_large_equal_scores(exponent, sign):
-    """Equal keys, scores of 2^44 (2^37 * 128 dims) times 2^exponent: the mean of the values. As the scores are equal to the last bit, they add nothing to
+    """Equal keys, scores of 101 * 2^37 (101 of 128 dims; times log2 e it has to be rounded) times 2^exponent: the mean of the values. As the scores are equal to the last bit, they add nothing to
     the bound."""
     for lens in ([40], [700], [3, 0, 2000]):
         q, p, table, n = _decode_case(len(lens), 8, 2, 128, 16, lens, 12)
         q.fill_(sign * 2.0 ** 37)
+        q[..., :27] = 0
         p.k.view(torch.uint8)[:] = torch.ones(1).to(F8).view(torch.uint8)
         p.k_scale.fill_(2.0 ** exponent)
         q0 = q * 0
@@ -449,6 +451,25 @@ def test_decode_is_the_same_run_after_run_on_streams_and_in_graphs():
     graphs[0][0].replay()
     torch.cuda.synchronize()
     assert torch.equal(graphs[0][1], CO.kv8_decode(q, p, table, n))
+    _no_kernel_error()
+
+
+@pytest.mark.gpu
+def test_decode_called_by_threads_that_share_a_stream():
+    args = []
+    for i, lens in enumerate(([900, 1, 64, 3000], [0, 2000, 1200, 5], [1, 1, 1, 4000], [700, 700, 700, 700])):
+        q, p, table, n = _decode_case(4, 16, 4, 64, 64, lens, 20 + i, width=70)
+        args.append((q.cuda(), _clone(p, "cuda"), table.cuda(), n.cuda()))
+    want = [CO.kv8_decode(*a) for a in args]
+    torch.cuda.synchronize()
+
+    def many(a):
+        torch.cuda.set_device(0)
+        return [CO.kv8_decode(*a) for _ in range(200)]
+    with ThreadPoolExecutor(len(args)) as pool:
+        got = list(pool.map(many, args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for outs, w in zip(got, want) for o in outs)
     _no_kernel_error()
 
 
