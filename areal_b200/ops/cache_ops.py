@@ -11,8 +11,8 @@ The engine takes this cache with ``NativeInferConfig.kv_cache_dtype = "float8_e4
 """
 from __future__ import annotations
 
-import ctypes
 import functools
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -254,7 +254,7 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
         with torch.cuda.device(dev):                 # whose stream it is that may be captured, and that the workspace belongs to
             return kv8_decode(q, pages, page_table, seq_lens, scale, out)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)             # half the host time of torch.empty
     if B == 0:
         return out
     st = q.stride()
@@ -337,8 +337,7 @@ def copy_pages(buffers: Sequence[tuple], src, dst, tokens=None) -> None:
     if dev < 0:
         return copy_pages_ref(buffers, src, dst, tokens)
     pairs = src + dst + (tokens if tokens is not None else [-1] * n)
-    flat, args = (ctypes.c_longlong * len(desc))(*desc), (ctypes.c_int * (3 * n))(*pairs)
-    _launch(dev, "ab2_copy_pages", ctypes.addressof(flat), len(buffers), ctypes.addressof(args), n)
+    _launch(dev, "ab2_copy_pages", struct.pack(f"{len(desc)}q", *desc), len(buffers), struct.pack(f"{3 * n}i", *pairs), n)
 
 
 def _ints(x) -> list:

@@ -81,7 +81,7 @@ struct Kv8Args {
 };
 
 // ------------------------------------------------------------------ append, one token for each row of the batch
-// One warp = (row, head, keys or values). The whole call is a few hundred KB at most and bound by latency: one load of the
+// One warp = (row, head, keys or values). The whole call is a few hundred KB at most and bound by latency (64 rows of 8 heads of 128: 2.1 us): one load of the
 // row, one of the scale, one store of each; a warp re-codes its block (8 KB at 64 x 128) only when the scale grows.
 template <int D>
 __global__ void __launch_bounds__(128)
@@ -135,7 +135,8 @@ kv8_append_row_kernel(const __grid_constant__ Kv8Args a, const int* __restrict__
 // ------------------------------------------------------------------ append, packed rows of several sequences
 // Sequence b brings rows cu[b] .. cu[b+1], its last ones: it is lens[b] long with them. One block = (page that gets rows, head,
 // keys or values): its rows (16 KB at 64 x 128) are read once into registers, their maximum decides the scale, and the codes go out
-// in one contiguous run. Which page a block has: the pages of sequence b are numbered from cu[b] / page_size + 2 b on, which
+// in one contiguous run. Bound by issue slots (62 % used) and the chain sequence, page, rows: 16384 rows of 8 heads of 128 take 16.2 us, 4.9 TB/s
+// of 79 MB. Which page a block has: the pages of sequence b are numbered from cu[b] / page_size + 2 b on, which
 // leaves room for the floor(n / page_size) + 2 that n rows can touch, so no scan over the batch is needed.
 template <int D, int NV>          // NV: 16-byte pieces of a thread = page_size * D / 8 / 128
 __global__ void __launch_bounds__(128, NV <= 8 ? 8 : 4)
@@ -210,7 +211,8 @@ kv8_append_page_kernel(const __grid_constant__ Kv8Args a, const int* __restrict_
 }
 
 // ------------------------------------------------------------------ attention of single tokens
-// o = softmax(scale * q K^T) V over the first lens[b] tokens, G query heads for each key/value head. Bound by the codes' bytes.
+// o = softmax(scale * q K^T) V over the first lens[b] tokens, G query heads for each key/value head. Bound by the codes' bytes: 256 x 2000..4001
+// tokens, 28 / 4 heads of 128, 139 us, 5.7 TB/s; 64 x 750..1500, 32 / 8 heads, 34 us, 4.1 TB/s, of which 8 us pass until the first tiles are here.
 //
 // Split: every (sequence, head) item is cut into units of U chunks of 64 tokens, U from the whole batch's tokens, whatever the lengths are.
 // Block i takes units i, i + grid, ...: about one each, so that taking them from a counter instead (SMs do not get equal shares of the
@@ -732,7 +734,8 @@ static int launch_kv8_decode(const Kv8Decode& a, int grid, cudaStream_t s) {
 // Copies pages src -> dst of up to four buffers in one launch: all planes (layers, keys and values, scales) of all pairs. A page of
 // a plane is `rows` runs of bytes, `row_stride` apart, of which the first tokens * token_bytes of each are copied (all of them where
 // tokens < 0). The pairs travel as kernel arguments, so a call needs no transfer. Bound by memory: 16 KB a block, 64 bytes a thread in flight
-// (32 KB and 128 bytes cost 15 % where the runs do not fill the blocks, and gain nothing on whole pages).
+// (32 KB and 128 bytes cost 15 % where the runs do not fill the blocks, and gain nothing on whole pages). 90 pages of 28 layers, 16 bits, 330 MB read
+// and 330 MB written: 101 us, 6.5 TB/s; 15 tails of 40 tokens of 36 layers in 8 bits: 10 us.
 constexpr int COPY_PAIRS = 256, COPY_BUFFERS = 4, COPY_PER = 4, COPY_BYTES = 256 * 16 * COPY_PER;
 struct CopyBuffer {
   unsigned char* base;

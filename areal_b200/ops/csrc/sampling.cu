@@ -19,10 +19,10 @@
 //   (4) Where even those bins are too full (thousands of equal logits, a long top-k), the range is cut again, until one value is left.
 // Then the blocks sum their kept weights by index, and the one in whose share u * W falls looks for the token.
 //
-// Measured (one B200, 151936 logits, device time): 1 row top-k 19 us, 64 rows of nuclei 99 us, 256 rows of all kinds 181 us. Reading the logits
+// Measured (one B200, 151936 logits, device time): 1 row top-k 19 us, 64 rows of nuclei 95 us, 256 rows of all kinds 172 us. Reading the logits
 // would take 0.1, 6 and 24 us: the time goes to a row's chain of steps (18 us for a usual row, 42 for a nucleus of tens of thousands), of which
 // 37 rows run at a time, as many as shared memory holds; inside them to issue slots, shared-memory atomics and the exchanges. (Read again
-// from the second-level cache instead, with clusters of four and twice the rows at a time, the same cases took 21, 99 and 178 us.)
+// from the second-level cache instead, with clusters of four and twice the rows at a time, the same cases took 21, 99 and 178 us where this took 19, 99 and 181.)
 #include <cmath>
 
 #include <cooperative_groups.h>
@@ -283,7 +283,8 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     auto clean = [](float x) { return fmaxf(x, -INFINITY); };               // NaN has no weight
     if (a.aligned) {
       const int n4 = n >> 2;
-      for (int i0 = tid; i0 < n4; i0 += SF_LOADS * SF_THREADS) {                        float4 v[SF_LOADS];
+      for (int i0 = tid; i0 < n4; i0 += SF_LOADS * SF_THREADS) {
+        float4 v[SF_LOADS];                                                 // all on their way before the first is used
 #pragma unroll
         for (int j = 0; j < SF_LOADS; ++j)
           v[j] = i0 + j * SF_THREADS < n4 ? __ldcs(reinterpret_cast<const float4*>(src) + i0 + j * SF_THREADS) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);

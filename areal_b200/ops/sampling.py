@@ -83,7 +83,7 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, inv_temp: torch.Tenso
     if ld < V:
         raise ValueError("rows of logits overlap")
     if out is None:
-        out = torch.empty(B, dtype=torch.int32, device=logits.device), torch.empty(B, device=logits.device)
+        out = torch.empty_like(top_k), torch.empty_like(u)
     _launch(dev, "ab2_sample_filtered", logits.data_ptr(), ld, B, V, u.data_ptr(), inv_temp.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
             min_p.data_ptr(), None if greedy is None else greedy.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
     return out
