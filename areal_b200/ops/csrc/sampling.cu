@@ -19,9 +19,9 @@
 //   (4) Where even those bins are too full (thousands of equal logits, a long top-k), the range is cut again, until one value is left.
 // Then the blocks sum their kept weights by index, and the one in whose share u * W falls looks for the token.
 //
-// Measured (one B200, 151936 logits, device time): 1 row top-k 19 us, 64 rows of nuclei 95 us, 256 rows of all kinds 172 us. Reading the logits
+// Measured (one B200, 151936 logits, device time): 1 row top-k 19 us, 64 rows of nuclei 93 us, 256 rows of all kinds 168 us. Reading the logits
 // would take 0.1, 6 and 24 us: the time goes to a row's chain of steps (18 us for a usual row, 42 for a nucleus of tens of thousands), of which
-// 37 rows run at a time, as many as shared memory holds; inside them to issue slots, shared-memory atomics and the exchanges. (Read again
+// 33 rows run at a time (two blocks on an SM, and whole clusters of eight in a GPC); inside them to issue slots, shared-memory atomics and the exchanges. (Read again
 // from the second-level cache instead, with clusters of four and twice the rows at a time, the same cases took 21, 99 and 178 us where this took 19, 99 and 181.)
 #include <cmath>
 
@@ -73,6 +73,7 @@ struct SampleShared {
   int ired[SF_WARPS];
   float thr;
   int ties, list_n, cut[4];
+  unsigned int arg[6];                 // of the row: inv_temp, top_p, min_p, u, top_k, greedy
 };
 
 // exp(d) for d <= 0 in 64 bits: exp(d) = 2^k * 2^(j/32) * exp(r), |r| <= ln 2 / 64, the last by its Taylor polynomial (table-driven
@@ -276,6 +277,12 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   pdl_trigger();
   const int begin = min(me * a.share, a.V), n = min(a.share, a.V - begin);       // this block's logits
   int buf = 0;                                                                   // set of the published values in use
+  // the row's arguments are read once, beside the logits, and the first block's are everyone's: all blocks take the same path
+  unsigned int arg = 0u;
+  if (me == 0 && tid < 6) {
+    const void* p = tid == 0 ? (const void*)a.inv_temp : tid == 1 ? a.top_p : tid == 2 ? a.min_p : tid == 3 ? a.u : tid == 4 ? (const void*)a.top_k : a.greedy;
+    if (p) arg = reinterpret_cast<const unsigned int*>(p)[row];
+  }
   // ---- the row into shared memory, its maximum
   float mx = -INFINITY;
   {
@@ -304,8 +311,10 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   for (int i = tid; i < SF_BINS; i += SF_THREADS) sh.hist[i] = 0u;
   if (tid < 32) sh.tab[tid] = a.tab[tid];
   if (tid == 0) sh.list_n = 0;
+  if (me == 0 && tid < 6) sh.arg[tid] = arg;
   sh.peak[tid] = mx;
   cl.sync();
+  if (me != 0 && tid < 6) sh.arg[tid] = cl.map_shared_rank(sh.arg, 0)[tid];
   float peaks[SF_MAX_CLUSTER], xmax = -INFINITY;                                 // every block looks at all threads' largest
 #pragma unroll
   for (int i = 0; i < SF_MAX_CLUSTER; ++i) {
@@ -328,16 +337,16 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     xmax = 0.f;
   }
   __syncthreads();
-  const float itf = a.inv_temp[row] >= 0.f ? fminf(a.inv_temp[row], 1e30f) : 0.f;
+  const float it_in = __uint_as_float(sh.arg[0]), tpf = __uint_as_float(sh.arg[1]), mpf = __uint_as_float(sh.arg[2]);
+  const bool greedy = sh.arg[5] != 0u;
+  int K = (int)sh.arg[4];
+  const float itf = it_in >= 0.f ? fminf(it_in, 1e30f) : 0.f;
   const double it = (double)itf, top = (double)xmax;
   const double top_it = top * it;
   // the same for every use of a logit: (x - max) * inv_temp in one rounding
   auto w_of = [&](float x) { return x == xmax ? 1.0 : weight(fma((double)x, it, -top_it), sh.tab); };
-  const bool greedy = a.greedy && a.greedy[row] != 0;
-  const float tpf = a.top_p[row];
-  const double top_p = (double)fmaxf(tpf, 0.f), min_p = (double)fminf(a.min_p[row], 1.f);
+  const double top_p = (double)fmaxf(tpf, 0.f), min_p = (double)fminf(mpf, 1.f);
   const bool by_mass = !greedy && tpf < 1.f;
-  int K = a.top_k[row];
   if (greedy || K <= 0 || K >= a.V) K = 0;
   const bool by_min = !greedy && min_p > 0.0;
 
@@ -414,7 +423,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       if (tid == 0) { sh.cut[0] = 0x7fffffff; sh.cut[1] = -1; }
       if (tid == m - 1) sh.red2[0] = run + w;
       __syncthreads();
-      const double all = sh.red2[0], goal = fmax((double)a.u[row], 0.0) * all;
+      const double all = sh.red2[0], goal = fmax((double)__uint_as_float(sh.arg[3]), 0.0) * all;
       if (tid < m) {
         double q[4] = {0.0, 0.0, 0.0, 0.0};
         for (int j = 0; j < m; j += 4) {
@@ -507,7 +516,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       mine += w[j];
     }
     run = block_scan(mine, sh.red, &sum);
-    const double goal = fmax((double)a.u[row], 0.0) * sum;
+    const double goal = fmax((double)__uint_as_float(sh.arg[3]), 0.0) * sum;
     int hit = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1273,7 +1282,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     sum += s;
     ties_left -= t;
   }
-  const double goal = fmax((double)a.u[row], 0.0) * sum;
+  const double goal = fmax((double)__uint_as_float(sh.arg[3]), 0.0) * sum;
   // the first block whose end passes the goal (the last one with any weight, should rounding leave none)
   const bool mine = my_sum > 0.0 && my_begin <= goal && (my_begin + my_sum > goal || me == last);
   if (!mine) return;
