@@ -506,7 +506,8 @@ class NativeInferConfig:
     # twice the tokens in the pool; head sizes 64 and 128, models on the paged cache
     kv_cache_dtype: str = "bfloat16"
     # Requests with top-k / top-p / min-p: "host" copies the step's logits and sorts them there, row by row (the draws of earlier versions);
-    # "device" samples them in one kernel, with draws of its own that depend on the request's seed and the position
+    # "device" samples them in one kernel, with draws of its own that depend on the request's seed and the position (stacks of the
+    # gated delta rule sample on the host either way)
     filtered_sampling: str = "host"
     use_cuda_graph: bool = True
     compute_dtype: str = "bfloat16"  # float32: matrices, activations and cache in 32 bits (mixer stacks only)

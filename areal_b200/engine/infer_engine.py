@@ -1247,7 +1247,10 @@ class NativeInferenceEngine(InferenceEngine):
         dev.copy_(host, non_blocking=True)
         fl = dev.view(torch.float32)
         OS.sample_filtered(logits, fl[3, :n], fl[2, :n], dev[1, :n], fl[4, :n], fl[5, :n], dev[0, :n], out=(self.s_out_tok[:n], self.s_out_lp[:n]))
-        return self._fetch_samples(n)
+        toks, lps = self._fetch_samples(n)
+        if any(toks[r] < 0 for r, _ in rows):            # (the host's draw refuses such a row too)
+            raise RuntimeError("a request's logits hold no number to draw by")
+        return toks, lps
 
     def _sample_cuda(self, logits: torch.Tensor, seqs: list[_Seq]):
         """Sampling for an ad-hoc list of sequences (prefill path)."""

@@ -167,6 +167,21 @@ def test_filtered_sampling_on_the_device(kw):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("place", ["host", "device"])
+def test_a_request_without_a_number_to_draw_by_is_an_error_and_no_token(place):
+    model = build_model(preset("tiny-qwen3"), dtype=torch.bfloat16, device="cuda", seed=5)
+    e = _engine(model, filtered_sampling=place)
+    s = IE._Seq(rid="a", tokens=[1], prompt_len=1, max_new=1, min_new=0, temperature=1.0, greedy=False, stop_ids=set(), ignore_eos=True, seed=1, top_p=0.9)
+    with torch.cuda.stream(e.stream):
+        logits = torch.randn(2, 1024, device="cuda")
+        assert min(e._sample_cuda(logits, [s, s])[0]) >= 0
+        logits[1] = float("nan")
+        with pytest.raises(RuntimeError):
+            e._sample_cuda(logits, [s, s])
+    e.destroy()
+
+
+@pytest.mark.gpu
 def test_device_and_host_filters_leave_the_same_distribution():
     """Next-token counts of many seeds on one prompt, both places: each token's share differs by less than five standard deviations."""
     model = build_model(preset("tiny-qwen3"), dtype=torch.bfloat16, device="cuda", seed=5)
