@@ -123,6 +123,17 @@ def test_the_statement_refuses_pages_and_lengths_out_of_range(page, lens):
         CO.kv8_append(*a)
 
 
+def test_decode_refuses_more_than_8192_sequences():
+    p = CO.QuantPages.empty(1, 1, 16, 64, "cpu")
+    for B in (8192, 8193):
+        q, table, lens = torch.zeros(B, 1, 64, dtype=torch.bfloat16), torch.zeros(B, 1, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
+        if B == 8192:
+            assert not CO.kv8_decode(q, p, table, lens).any()
+        else:
+            with pytest.raises(ValueError):
+                CO.kv8_decode(q, p, table, lens)
+
+
 @pytest.mark.parametrize("what", ["dtype", "group", "batch", "dim", "out", "table", "pages"])
 def test_decode_refuses(what):
     p = CO.QuantPages.empty(4, 2, 16, 64, "cpu")
@@ -451,6 +462,42 @@ def test_decode_is_the_same_run_after_run_on_streams_and_in_graphs():
     graphs[0][0].replay()
     torch.cuda.synchronize()
     assert torch.equal(graphs[0][1], CO.kv8_decode(q, p, table, n))
+    _no_kernel_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [129, 1000, 8192])
+def test_decode_of_many_short_contexts(B):
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 30, (B,), generator=g).tolist()
+    lens[B // 2] = 900
+    _check_decode(*_decode_case(B, 2, 1, 64, 16, lens, B))
+
+
+@pytest.mark.gpu
+def test_pages_whose_offsets_pass_32_bits():
+    """A cache of 4.3 GB of keys: append, attention and copies on its last pages do what they do on a small one with the same pages in front."""
+    P, Hkv, ps, D, n = 66000, 8, 64, 128, 6
+    big, small = CO.QuantPages.empty(P, Hkv, ps, D, "cuda"), CO.QuantPages.empty(n, Hkv, ps, D, "cuda")
+    assert big.k.numel() > 2 ** 32
+    table = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([150, 70], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 150, 220], dtype=torch.int32, device="cuda")
+    k, v, q = (torch.randn(m, h, D, device="cuda").bfloat16() for m, h in ((220, Hkv), (220, Hkv), (2, 4 * Hkv)))
+    outs = []
+    for p, t in ((small, table), (big, table + (P - n))):
+        CO.kv8_append(k, v, p, t, lens, cu)
+        CO.kv8_append(k[:2], v[:2], p, t, lens + 1)
+        outs.append(CO.kv8_decode(q, p, t, lens + 1))
+    assert torch.equal(outs[0], outs[1])
+    tail = lambda x: (x.view(torch.uint8) if x.dtype == F8 else x)[P - n:]                     # noqa: E731
+    for x, y in zip((small.k, small.v, small.k_scale, small.v_scale), (big.k, big.v, big.k_scale, big.v_scale)):
+        assert torch.equal(x.view(torch.uint8) if x.dtype == F8 else x, tail(y))
+    codes = big.k.view(torch.uint8)
+    assert not codes[:P - n].any()
+    CO.copy_pages([(codes, 0, 2), (big.k_scale, 0, None)], [P - 6, P - 5, P - 3], [1, P - 1, 0], [64, 33, 1])
+    for s, d, m in ((P - 6, 1, 64), (P - 5, P - 1, 33), (P - 3, 0, 1)):
+        assert torch.equal(codes[s, :, :m], codes[d, :, :m]) and torch.equal(big.k_scale[s], big.k_scale[d]) and not codes[d, :, m:].any()
     _no_kernel_error()
 
 
