@@ -225,11 +225,15 @@ kv8_append_page_kernel(const __grid_constant__ Kv8Args a, const int* __restrict_
 //   O^T[D dims, 8 heads] += V^T P^T: rows (dims) may stand in any order too, so a thread's 16 contiguous dims of four tokens are
 //     paired by byte permutes; P^T comes from S^T by an 8 x 8 transpose between registers.
 // The 16-byte pieces of a 128-byte line stand where their number is xor-ed with the line's, so that both patterns of reads are free of
-// bank conflicts. e4m3 converts to fp16 exactly; q is divided by a power of two for its head (exact), P is rounded to fp16 (11 bits,
-// half a step 2^-12) as e^x scaled so that the largest seen lies between 2^9 and 2^15 (the running maximum only moves when a score leaves
-// that range, so that shares down to 2^-23 of the largest keep all bits), and both sums are fp32.
+// bank conflicts. e4m3 converts to fp16 exactly; q is divided by a power of two for its head (exact), and both sums are fp32.
+// P is rounded to fp16 (half a step 2^-11) and multiplies codes, so it holds the page's value scale: probability times scale, what the token can add to
+// the result, as 2^(x + log2 scale - d). The largest of it seen lies between 2^8 and 2^15 (m and d only move when a token leaves that range), so that all
+// down to 2^-22 of the largest keep all bits, whatever the scales are and in whatever order the pages come. The sum of the probabilities
+// alone has a reference of its own, m: a token may have all the weight and add next to nothing, or the other way round. m and d are whole
+// numbers, d counted from m: moving them multiplies by powers of two, and neither rounds where scores are large.
 constexpr int KV8_CHUNK = 64, KV8_MOST_ROWS = 8192;
 constexpr int KV8_LEAST = 4;        // chunks of the smallest unit: what a split saves of so short an item, the join costs
+constexpr float KV8_LOW = -300.f;   // below every d: a scale is 2^-100 or more
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -269,9 +273,17 @@ __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&h);
+// log2 of a scale; a power of two gives a whole number.
+__device__ __forceinline__ float log2_scale(float s) {
+  const int bits = __float_as_int(s);
+  const float e = (float)((bits >> 23) - 127);
+  if (s > 0.f) return bits & 0x7fffff ? e + __log2f(__int_as_float((bits & 0x7fffff) | 0x3f800000)) : e;
+  return s == 0.f ? -INFINITY : NAN;
+}
+// a * 2^d in two steps: 2^d alone may be out of range where the product is not.
+__device__ __forceinline__ float times_pow2(float a, float d) {
+  const int k = (int)fminf(fmaxf(d, -250.f), 250.f), h = k >> 1;
+  return a * pow2i(h) * pow2i(k - h);
 }
 
 struct Kv8Decode {
@@ -280,7 +292,8 @@ struct Kv8Decode {
   const float *ks, *vs;
   const int *table, *lens;
   __nv_bfloat16* out;
-  float *part_o, *part_ml;      // [slots][HP][D], [slots][HP][2]: units of items that are split
+  float* part_o;                // [slots][HP][D]: units of items that are split, divided by 2^(m + d)
+  float4* part_ml;              // [slots][HP]: m, the sum of probabilities divided by 2^m, d
   int2* meta;                   // [B] units of an item of the sequence, and its first slot
   int* err;
   int B, Hq, Hkv, G, groups, page_size, page_bits, width, num_pages;
@@ -313,7 +326,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
   extern __shared__ __align__(128) unsigned char dsm[];       // four rings; where a unit ends, each holds its warp's result [HP][D + 4]
   float* mm = reinterpret_cast<float*>(dsm + 4 * Cfg::RING);  // [4][HP]
   float* ml = mm + 4 * HP;                                    // [4][HP]
-  int* units = reinterpret_cast<int*>(ml + 4 * HP);           // [B + 1] units of one head before sequence b
+  float* md = ml + 4 * HP;                                    // [4][HP]
+  int* units = reinterpret_cast<int*>(md + 4 * HP);           // [B + 1] units of one head before sequence b
   int* slots = units + a.B + 1;                               // [B + 1] those of split items only
   __shared__ int wsum[2][4];
   __shared__ float s_scale[4][S][2];                          // scales of the tiles in the rings
@@ -479,17 +493,17 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
       qs[t][1] = __shfl_sync(0xffffffffu, f, 8 * tq + 4);
     }
 
-    float o[NT][KS][4], m_run[NT][2], l_run[NT][2], v_ref = 0.f;
+    float o[NT][KS][4], m_run[NT][2], l_run[NT][2], d_run[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int i = 0; i < KS; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
       m_run[t][0] = m_run[t][1] = -3e38f;                       // below every finite score, and a difference of two such is no NaN
       l_run[t][0] = l_run[t][1] = 0.f;
+      d_run[t][0] = d_run[t][1] = KV8_LOW;
     }
 
-    float v_last = 0.f;
-    uint32_t ratio = 0u;                                        // scale of this page's values over v_ref, as two fp16
+    float v_last = -1.f, lv = 0.f;                              // value scale of the page, and its log2
     auto work = [&](int i) {
       const float kscale = s_scale[warp][sc_out][0], vscale = s_scale[warp][sc_out][1];
       sc_out = sc_out == S - 1 ? 0 : sc_out + 1;
@@ -528,7 +542,11 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) v[r][c] = 0u;
       }
-      // x = score - running maximum; both of a head's tokens. The product is rounded as the maximum's was: with one rounding for both steps, large
+      if (vscale != v_last) {                                   // another page
+        v_last = vscale;
+        lv = log2_scale(vscale);
+      }
+      // x = score - m; both of a head's tokens. The product is rounded as the maximum's was: with one rounding for both steps, large
       // scores (2^24 and more) would be off by the rounding of the maximum's product, whole powers of two.
       float x[NT][4], f[NT][2];
       bool grow = false;
@@ -543,7 +561,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
           if (gq >= left) x[t][0] = x[t][1] = -INFINITY;
           if (gq + 8 >= left) x[t][2] = x[t][3] = -INFINITY;
         }
-        grow |= fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])) > 15.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) grow |= fmaxf(x[t][e], x[t][e + 2]) > fminf(15.f, 15.f - (lv - d_run[t][e]));
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -556,30 +575,23 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
             float top = fmaxf(in0 ? __fmul_rn(s[t][e], f[t][e]) : -INFINITY, in1 ? __fmul_rn(s[t][e + 2], f[t][e]) : -INFINITY);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - 9.f;              // the largest becomes 2^9
-            if (top > m_run[t][e]) {
-              const float al = fast_exp2(m_run[t][e] - top);
-              m_run[t][e] = top;
-              x[t][e] = in0 ? __fmul_rn(s[t][e], f[t][e]) - top : -INFINITY;
-              x[t][e + 2] = in1 ? __fmul_rn(s[t][e + 2], f[t][e]) - top : -INFINITY;
-              l_run[t][e] *= al;
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float m = fmaxf(m_run[t][e], ceilf(top) - 9.f);                       // the largest probability becomes 2^8 to 2^9
+            const float d_old = d_run[t][e] - (m - m_run[t][e]);                        // the same unit of the sums, counted from the new m
+            const float d = fmaxf(fmaxf(d_old, ceilf(top - m + lv) - 9.f), KV8_LOW);    // and the largest share of the result too
+            if (m > m_run[t][e]) {
+              l_run[t][e] *= fast_exp2(m_run[t][e] - m);
+              m_run[t][e] = m;
+              x[t][e] = in0 ? __fmul_rn(s[t][e], f[t][e]) - m : -INFINITY;
+              x[t][e + 2] = in1 ? __fmul_rn(s[t][e + 2], f[t][e]) - m : -INFINITY;
+            }
+            d_run[t][e] = d;
+            if (d > d_old) {
+              const float al = fast_exp2(d_old - d);
 #pragma unroll
               for (int i2 = 0; i2 < KS; ++i2) { o[t][i2][e] *= al; o[t][i2][e + 2] *= al; }
             }
           }
-      }
-      if (vscale != v_last) {                                   // another page
-        v_last = vscale;
-        if (vscale > v_ref) {                                   // whose values have a larger scale than those before
-          const float r = v_ref / vscale;
-          v_ref = vscale;
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i2 = 0; i2 < KS; ++i2) { o[t][i2][0] *= r; o[t][i2][1] *= r; o[t][i2][2] *= r; o[t][i2][3] *= r; }
-        }
-        const float r = v_ref > 0.f ? vscale / v_ref : 0.f;
-        ratio = pack_f16(r, r);
       }
       uint32_t p0[NT], p1[NT];
 #pragma unroll
@@ -587,8 +599,9 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
         const float e0 = fast_exp2(x[t][0]), e1 = fast_exp2(x[t][1]), e2 = fast_exp2(x[t][2]), e3 = fast_exp2(x[t][3]);
         l_run[t][0] += e0 + e2;
         l_run[t][1] += e1 + e3;
-        p0[t] = transpose8x8(mul_f16x2(pack_f16(e0, e1), ratio));
-        p1[t] = transpose8x8(mul_f16x2(pack_f16(e2, e3), ratio));
+        const float c0 = lv - d_run[t][0], c1 = lv - d_run[t][1];
+        p0[t] = transpose8x8(pack_f16(fast_exp2(x[t][0] + c0), fast_exp2(x[t][1] + c1)));
+        p1[t] = transpose8x8(pack_f16(fast_exp2(x[t][2] + c0), fast_exp2(x[t][3] + c1)));
       }
 #pragma unroll
       for (int j = 0; j < KS; ++j) {                            // dims gq * D/8 + 2 j and + 2 j + 1
@@ -622,10 +635,11 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
         if (gq == 0) {
           mm[warp * HP + hd] = m_run[t][e];
           ml[warp * HP + hd] = l;
+          md[warp * HP + hd] = d_run[t][e];
         }
 #pragma unroll
         for (int j = 0; j < KS; ++j)
-          *reinterpret_cast<float2*>(&mo[hd * (D + 4) + gq * (D / 8) + 2 * j]) = make_float2(o[t][j][e] * v_ref, o[t][j][e + 2] * v_ref);
+          *reinterpret_cast<float2*>(&mo[hd * (D + 4) + gq * (D / 8) + 2 * j]) = make_float2(o[t][j][e], o[t][j][e + 2]);
       }
     }
     __syncthreads();
@@ -635,18 +649,21 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
       float mx = mm[g];
 #pragma unroll
       for (int w = 1; w < 4; ++w) mx = fmaxf(mx, mm[w * HP + g]);
+      float dx = mm[g] - mx + md[g];                            // the warps' units, counted from the largest m
+#pragma unroll
+      for (int w = 1; w < 4; ++w) dx = fmaxf(dx, mm[w * HP + g] - mx + md[w * HP + g]);
       float l = 0.f, acc = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float f = fast_exp2(mm[w * HP + g] - mx);
-        l += ml[w * HP + g] * f;
-        acc += reinterpret_cast<const float*>(dsm + w * Cfg::RING)[g * (D + 4) + d] * f;
+        const float below = mm[w * HP + g] - mx;
+        l += ml[w * HP + g] * fast_exp2(below);
+        acc += reinterpret_cast<const float*>(dsm + w * Cfg::RING)[g * (D + 4) + d] * fast_exp2(below + md[w * HP + g] - dx);
       }
       if (np == 1) {
-        a.out[((size_t)b * a.Hq + h * a.G + g0 + g) * D + d] = __float2bfloat16(acc / l);
+        a.out[((size_t)b * a.Hq + h * a.G + g0 + g) * D + d] = __float2bfloat16(times_pow2(acc / l, dx));
       } else {
         a.part_o[((size_t)slot * HP + g) * D + d] = acc;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)slot * HP + g) * 2) = make_float2(mx, l);
+        if (d == 0) a.part_ml[(size_t)slot * HP + g] = make_float4(mx, l, dx, 0.f);
       }
     }
     __syncthreads();                                            // the rings are free for the next unit
@@ -658,7 +675,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
 template <int D, int NT>
 __global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ Kv8Decode a) {
   constexpr int HP = 8 * NT, PER = D / 32;
-  __shared__ float so[4][D], sm[4], sl[4];
+  __shared__ float so[4][D], sm[4], sl[4], sd[4];
   pdl_wait();
   pdl_trigger();
   const int2 meta = a.meta[blockIdx.x];
@@ -667,15 +684,18 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ K
   for (int hq = blockIdx.y; hq < a.Hq; hq += gridDim.y) {
     const int h = hq / a.G, gh = hq - h * a.G, grp = gh / 16, g = gh - grp * 16;
     const size_t first = (size_t)(meta.y + (h * a.groups + grp) * np);
-    float mx = -INFINITY, l = 0.f, acc[PER];
+    float mx = -INFINITY, l = 0.f, dx = -INFINITY, acc[PER];   // acc: divided by 2^(mx + dx)
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
     for (int i0 = warp; i0 < np; i0 += 128) {                   // units i0, i0 + 4, ...: 32 of them
       const int i = i0 + 4 * lane, n = min(32, (np - i0 + 3) / 4);
-      const float2 p = i < np ? *reinterpret_cast<const float2*>(a.part_ml + ((first + i) * HP + g) * 2) : make_float2(-INFINITY, 0.f);
-      const float m = fmaxf(mx, warp_max(p.x)), f0 = fast_exp2(mx - m), f = fast_exp2(p.x - m);
+      const float4 p = i < np ? a.part_ml[(first + i) * HP + g] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      const float m = fmaxf(mx, warp_max(p.x));
+      l = l * fast_exp2(mx - m) + p.y * fast_exp2(p.x - m);
+      const float d_old = mx - m + dx, d_own = p.x - m + p.z, d = fmaxf(d_old, warp_max(d_own));
+      const float f0 = fast_exp2(d_old - d), f = fast_exp2(d_own - d);
       mx = m;
-      l = l * f0 + p.y * f;
+      dx = d;
 #pragma unroll
       for (int e = 0; e < PER; ++e) acc[e] *= f0;
       for (int j0 = 0; j0 < n; j0 += 8) {
@@ -697,15 +717,22 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ K
     l = warp_sum(l);
 #pragma unroll
     for (int e = 0; e < PER; ++e) so[warp][lane * PER + e] = acc[e];
-    if (lane == 0) { sm[warp] = mx; sl[warp] = l; }
+    if (lane == 0) { sm[warp] = mx; sl[warp] = l; sd[warp] = dx; }
     __syncthreads();
     mx = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     l = 0.f;
+    dx = -INFINITY;
     float f[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) { f[w] = fast_exp2(sm[w] - mx); l += sl[w] * f[w]; }
+    for (int w = 0; w < 4; ++w) {
+      l += sl[w] * fast_exp2(sm[w] - mx);
+      f[w] = sm[w] - mx + sd[w];
+      dx = fmaxf(dx, f[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) f[w] = fast_exp2(f[w] - dx);
     for (int d = threadIdx.x; d < D; d += 128)
-      a.out[((size_t)b * a.Hq + hq) * D + d] = __float2bfloat16((so[0][d] * f[0] + so[1][d] * f[1] + so[2][d] * f[2] + so[3][d] * f[3]) / l);
+      a.out[((size_t)b * a.Hq + hq) * D + d] = __float2bfloat16(times_pow2((so[0][d] * f[0] + so[1][d] * f[1] + so[2][d] * f[2] + so[3][d] * f[3]) / l, dx));
     __syncthreads();
   }
 }
@@ -715,7 +742,7 @@ static std::mutex g_kv8_pair;
 
 template <int D, int NT>
 static int launch_kv8_decode(const Kv8Decode& a, int grid, cudaStream_t s) {
-  constexpr int HP = 8 * NT, RING = 4 * Kv8Cfg<D, NT>::RING + 8 * HP * 4;
+  constexpr int HP = 8 * NT, RING = 4 * Kv8Cfg<D, NT>::RING + 12 * HP * 4;
   const int smem = RING + 2 * (a.B + 1) * 4;
   auto kern = kv8_decode_kernel<D, NT>;
   static ab2host::DevState st;
@@ -852,7 +879,7 @@ long long ab2_kv8_decode_workspace(int B, int Hq, int Hkv, int D, int page_size,
   if (B <= 0 || Hkv <= 0 || Hq % Hkv) return 0;
   const int G = Hq / Hkv, HP = G <= 8 ? 8 : 16;
   const long long slots = 2LL * kv8_grid(B, Hq, Hkv, width, page_size, ab2_num_sms());
-  return slots * HP * (D + 2) * 4 + (long long)B * 8;
+  return slots * HP * (D + 4) * 4 + (long long)B * 8;
 }
 
 // q [B, Hq, D] bf16 (rows q_stride elements apart, heads dense), out [B, Hq, D] dense; cache and table as above; lens [B]. Calls that
@@ -876,8 +903,8 @@ int ab2_kv8_decode(const void* q, const void* kc, const void* vc, const void* ks
   a.scale_log2 = scale * 1.4426950408889634f; a.q_stride = q_stride; a.err = ab2host::error_flag();
   const int HP = G <= 8 ? 8 : 16;
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + 2LL * grid * HP * D;
-  a.meta = (int2*)(a.part_ml + 2LL * grid * HP * 2);
+  a.part_ml = (float4*)(a.part_o + 2LL * grid * HP * D);
+  a.meta = (int2*)(a.part_ml + 2LL * grid * HP);
   cudaStream_t s = (cudaStream_t)stream;
   if (D == 128) return G <= 8 ? launch_kv8_decode<128, 1>(a, grid, s) : launch_kv8_decode<128, 2>(a, grid, s);
   return G <= 8 ? launch_kv8_decode<64, 1>(a, grid, s) : launch_kv8_decode<64, 2>(a, grid, s);

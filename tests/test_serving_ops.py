@@ -412,6 +412,68 @@ def test_decode_of_large_equal_scores(exponent, sign):
         assert torch.all((out.double() - ref).abs() <= _decode_bound(q0, p, table, n, 1.0, ref))
 
 
+def _shares_bound(q, p, table, lens, scale, ref):
+    """As :func:`_decode_bound`, but what a probability loses below fp16's normal range is bounded by what the tokens add to the result, not by the largest value
+    there is: probability times value scale is held to half of fp16's smallest step, 2^-25, in units in which the largest of them is 2^8 or
+    more, and multiplies a code."""
+    out = torch.zeros_like(ref)
+    B, Hq, D = q.shape
+    Hkv, ps = p.k.shape[1:3]
+    for b, n in enumerate(lens.tolist()):
+        if n <= 0:
+            continue
+        pg = table[b, :-(-n // ps)].long()
+        codes = p.v.view(torch.uint8)[pg].view(F8).double().transpose(0, 1).reshape(Hkv, -1, D)[:, :n].abs()
+        K = (p.k.view(torch.uint8)[pg].view(F8).double() * p.k_scale[pg].double()[:, :, None, None]).transpose(0, 1).reshape(Hkv, -1, D)[:, :n]
+        vs = p.v_scale[pg].double().t().repeat_interleave(ps, 1)[:, None, :n]
+        qb = q[b].double().view(Hkv, -1, D)
+        pr = torch.softmax(torch.einsum("hgd,htd->hgt", qb, K) * scale, -1)
+        size = torch.einsum("hgd,htd->hgt", qb.abs(), K.abs()) * abs(scale)
+        ds = 2 * (D + 4) * 2.0 ** -24 * size.amax(-1, keepdim=True)
+        mean = torch.einsum("hgt,htd->hgd", pr * vs, codes)
+        low = 2.0 ** -33 * (pr * vs).amax(-1, keepdim=True) * codes.sum(1)[:, None]
+        out[b] = ((2.0 ** -11 + 2.0 ** -18 + ds) * mean + low).reshape(Hq, D)
+    return out + 2.0 ** -8 * (ref.abs() + out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["large first", "small first", "in turn"])
+@pytest.mark.parametrize("apart", [10, 24, 30, 60, 120, 220])
+@pytest.mark.parametrize("Hq,Hkv,D,ps,n", [(8, 2, 128, 64, 256), (8, 2, 64, 16, 250), (16, 1, 128, 16, 130), (4, 2, 64, 128, 256), (8, 2, 128, 64, 9000), (24, 2, 64, 32, 5000)])
+def test_decode_of_pages_whose_value_scales_are_far_apart(Hq, Hkv, D, ps, n, apart, order):
+    """Pages of two value scales, 2^apart from one another. The tokens on the large ones have less weight, by the square root of 2^apart (their values
+    decide the result and the others the sum of the weights), by 2^apart and by its square (they have no part in anything)."""
+    P = -(-n // ps)
+    large = torch.arange(P) < P // 2 if order == "large first" else torch.arange(P) >= -(-P // 2) if order == "small first" else torch.arange(P) // (64 // min(ps, 64)) % 2 == 0
+    for much in (0.5, 1.0, 2.0):
+        q, p, table, lens = _decode_case(1, Hq, Hkv, D, ps, [n], apart)
+        pages = table[0, :P].long()
+        p.k.copy_((torch.randn(p.k.shape, generator=torch.Generator().manual_seed(n)) * 0.05).to(F8))
+        p.k_scale.fill_(1.0)
+        q[..., 0] = 1.0
+        raw = p.k.view(torch.uint8)
+        raw[pages[large], :, :, 0] = torch.tensor([-much * apart * math.log(2)]).to(F8).view(torch.uint8)
+        p.v_scale[pages] = torch.where(large, 2.0 ** (apart - 100), 2.0 ** -100)[:, None].expand(P, Hkv).float()
+        ref = CO.kv8_decode_ref(q, p, table, lens, 1.0)
+        out = CO.kv8_decode(q.cuda(), _clone(p, "cuda"), table.cuda(), lens.cuda(), 1.0).cpu()
+        _no_kernel_error()
+        assert torch.all((out.double() - ref).abs() <= _shares_bound(q, p, table, lens, 1.0, ref)), (much, float(((out.double() - ref).abs() / ref.abs()).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 200, 6000])
+def test_decode_of_the_largest_and_smallest_values(n):
+    """Values next to bf16's largest number and to a scale's smallest: the result lies among them and is a number."""
+    for e in (119, -100):
+        q, p, table, lens = _decode_case(2, 8, 2, 128, 64, [n, n // 2], 31)
+        p.v.copy_((torch.rand(p.v.shape, generator=torch.Generator().manual_seed(n)) * 100 + 150).to(F8))          # below 2^8: values below 2^127
+        p.v_scale.fill_(2.0 ** e)
+        ref = CO.kv8_decode_ref(q, p, table, lens)
+        out = CO.kv8_decode(q.cuda(), _clone(p, "cuda"), table.cuda(), lens.cuda()).cpu()
+        _no_kernel_error()
+        assert torch.all((out.double() - ref).abs() <= _shares_bound(q, p, table, lens, 128 ** -0.5, ref))
+
+
 @pytest.mark.gpu
 def test_decode_takes_parts_of_a_projection_and_reports_bad_tables():
     q, p, table, n = _decode_case(5, 8, 2, 64, 32, [40, 1, 200, 0, 64], 4)
