@@ -42,6 +42,7 @@ constexpr int SF_LOADS = 10;           // 16-byte loads of a thread on their way
 constexpr int SF_GUESS = 256;          // tokens of a nucleus that is tried without a histogram of the row
 constexpr int SF_MAX_CLUSTER = 8;
 constexpr float SF_PER_NAT = 64.f;
+constexpr double SF_NONE = 0x1p-1015;  // weights above it count: the smallest is e^-700.0005, above 2^-1010; 2^19 tokens without weight sum to less than 2^-1023
 
 struct SampleArgs {
   const float* logits;
@@ -77,7 +78,8 @@ struct SampleShared {
 };
 
 // exp(d) for d <= 0 in 64 bits: exp(d) = 2^k * 2^(j/32) * exp(r), |r| <= ln 2 / 64, the last by its Taylor polynomial (table-driven
-// exponentials after P. T. P. Tang, 1989; relative error below 2e-12). Zero below e^-700.
+// exponentials after P. T. P. Tang, 1989; relative error below 2e-12). From -(700 + 2^-11) down a token has no weight: what is returned there is below 2^-1042 (its
+// high word is cleared; clearing the low one too cost 8 %), in sums nothing, and below SF_NONE however many there are.
 __device__ __forceinline__ double weight(double d, const double* tab) {
   const double big = 6755399441055744.0;                       // 1.5 * 2^52: adding it rounds to a whole number
   const double t = fma(d, 46.166241308446828, big);            // 32 / ln 2
@@ -88,9 +90,9 @@ __device__ __forceinline__ double weight(double d, const double* tab) {
   p = fma(p, r, 1.0);
   p = fma(p, r, 1.0);
   const double w = p * tab[k & 31];
-  // e^-700 and less (the high word of a negative number rises as it falls; minus infinity and NaN are above them all): zero
+  // (the high word of a negative number rises as it falls, 2^-11 at a time here; minus infinity and NaN are above them all)
   const bool gone = (unsigned int)__double2hiint(d) > 0xc085e000u;
-  return __hiloint2double(gone ? 0 : __double2hiint(w) + ((k >> 5) << 20), __double2loint(w));      // (below 1e-307 where gone)
+  return __hiloint2double(gone ? 0 : __double2hiint(w) + ((k >> 5) << 20), __double2loint(w));
 }
 // Order-preserving map of floats to unsigned.
 __device__ __forceinline__ unsigned int key_of(float x) {
@@ -416,14 +418,14 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       const double w = tid < k ? w_of(float_of((unsigned int)(e >> 32))) : 0.0;
       double sum;
       const double run = block_scan(w, sh.red, &sum, (cnt + 31) >> 5);
-      const bool kept = w > 0.0 && (!by_mass || run <= top_p * (K > 0 ? sum : total)) && w >= min_p;
+      const bool kept = w > SF_NONE && (!by_mass || run <= top_p * (K > 0 ? sum : total)) && w >= min_p;
       const int m = max(1, __syncthreads_count(kept));                            // its barrier also ends the use of hist
       const int index = (int)(0xffffffffu - (unsigned int)e);
       if (tid < m) ws[tid] = w;
       if (tid == 0) { sh.cut[0] = 0x7fffffff; sh.cut[1] = -1; }
       if (tid == m - 1) sh.red2[0] = run + w;
       __syncthreads();
-      const double all = sh.red2[0], goal = fmax((double)__uint_as_float(sh.arg[3]), 0.0) * all;
+      const double all = sh.red2[0], goal = fmax((double)__uint_as_float(sh.arg[3]) * all, SF_NONE);
       if (tid < m) {
         double q[4] = {0.0, 0.0, 0.0, 0.0};
         for (int j = 0; j < m; j += 4) {
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = 4 * tid + j;
-      if (i < k && w[j] > 0.0 && (!by_mass || run <= top_p * all) && w[j] >= min_p) ++kept;
+      if (i < k && w[j] > SF_NONE && (!by_mass || run <= top_p * all) && w[j] >= min_p) ++kept;
       run += w[j];
     }
     int m;
@@ -516,7 +518,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       mine += w[j];
     }
     run = block_scan(mine, sh.red, &sum);
-    const double goal = fmax((double)__uint_as_float(sh.arg[3]), 0.0) * sum;
+    const double goal = fmax((double)__uint_as_float(sh.arg[3]) * sum, SF_NONE);
     int hit = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1278,13 +1280,13 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     const int t = min(sh.pub_int[buf][i], ties_left);
     const double s = sh.pub_sum[buf][i] + t * w_tie;
     if (i == me) { my_begin = sum; my_sum = s; my_ties = ties_left; }
-    if (s > 0.0) last = i;
+    if (s > SF_NONE) last = i;
     sum += s;
     ties_left -= t;
   }
-  const double goal = fmax((double)__uint_as_float(sh.arg[3]), 0.0) * sum;
+  const double goal = fmax((double)__uint_as_float(sh.arg[3]) * sum, SF_NONE);      // (above nothing: u may be 0)
   // the first block whose end passes the goal (the last one with any weight, should rounding leave none)
-  const bool mine = my_sum > 0.0 && my_begin <= goal && (my_begin + my_sum > goal || me == last);
+  const bool mine = my_sum > SF_NONE && my_begin <= goal && (my_begin + my_sum > goal || me == last);
   if (!mine) return;
   for (int g = warp; g < segs; g += SF_WARPS) {
     double s = 0.0;
@@ -1328,7 +1330,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       const double t = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += t;
     }
-    const unsigned int some = __ballot_sync(0xffffffffu, own > 0.0), hit = __ballot_sync(0xffffffffu, own > 0.0 && run + s > goal);
+    const unsigned int some = __ballot_sync(0xffffffffu, own > SF_NONE), hit = __ballot_sync(0xffffffffu, own > SF_NONE && run + s > goal);
     if (some) {
       const int from = hit ? __ffs(hit) - 1 : 31 - __clz(some);
       sg = g0 + from;
@@ -1357,7 +1359,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       const double t = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += t;
     }
-    const unsigned int some = __ballot_sync(0xffffffffu, w > 0.0), hit = __ballot_sync(0xffffffffu, w > 0.0 && run + s > goal);
+    const unsigned int some = __ballot_sync(0xffffffffu, w > SF_NONE), hit = __ballot_sync(0xffffffffu, w > SF_NONE && run + s > goal);
     if (some) {
       const int from = hit ? __ffs(hit) - 1 : 31 - __clz(some);
       tok = begin + i0 + from;

@@ -13,6 +13,7 @@ from . import lib as _lib
 from .cache_ops import _launch, _need
 
 _V, _I, _L = _lib.c_void_p, _lib.c_int, _lib.c_ll
+NO_WEIGHT = -(700 + 2.0 ** -11)          # from here down a token has no weight: e^-700 is next to the smallest number of 64 bits
 MAX_VOCAB = 8 * 49152        # the kernel holds a row in the shared memory of eight SMs
 
 
@@ -29,7 +30,7 @@ def sample_filtered_ref(logits, u, inv_temp, top_k, top_p, min_p, greedy=None):
         if top == float("-inf"):
             continue
         it = float(inv_temp[b])
-        w = torch.where(x == top, torch.ones_like(x), torch.where(x == float("-inf"), torch.zeros_like(x), torch.exp((x - top) * it)))
+        w = torch.where(x == top, torch.ones_like(x), torch.where((x == float("-inf")) | ((x - top) * it <= NO_WEIGHT), torch.zeros_like(x), torch.exp((x - top) * it)))
         if greedy is not None and int(greedy[b]):
             tok[b], lp[b] = int(order[0]), -torch.log(w.sum())
             continue
@@ -58,7 +59,7 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, inv_temp: torch.Tenso
     ``min_p`` keeps ``w_i >= min_p``. The token is the lowest index at which the kept weights, summed by index, pass ``u`` times their
     sum ``W`` (``u`` in [0, 1)); its log-prob is ``ln(w / W)``. A row with ``greedy`` set takes the first of the order, with its log-prob
     over all tokens. ``top_k <= 0`` (or >= V), ``top_p >= 1`` and ``min_p <= 0`` switch a filter off; ``inv_temp`` is positive. Logits of minus
-    infinity and NaN have no weight; infinite ones share all of it. A row in which nothing has weight gives token -1 and minus infinity.
+    infinity and NaN have no weight, nor have those more than 700 nats below the largest; infinite ones share all of it. A row in which nothing has weight gives token -1 and minus infinity.
 
     ``u``, ``inv_temp``, ``top_p``, ``min_p``: fp32 ``[B]``; ``top_k``, ``greedy``: int32 ``[B]``. Rows of logits may lie apart (a slice of a wider
     tensor). At most 393216 tokens in the vocabulary on CUDA."""

@@ -696,6 +696,43 @@ def test_sampling_rows_at_the_edges():
         assert int(got) == want
 
 
+def _masked_rows(V, low, offset, kind, u, **filters):
+    """Rows in which all but a window of tokens stand at ``low`` (its first two rows: the window at the front and at the end)."""
+    g = torch.Generator().manual_seed(V)
+    B = 6
+    x = torch.full((B, V), low)
+    n = max(1, min(V // 3, 5000) if kind == "long" else min(V // 3, 90))
+    for b in range(B):
+        at = (0, V - n)[b] if b < 2 else int(torch.randint(0, V - n + 1, (1,), generator=g))
+        x[b, at:at + n] = (torch.randn(n, generator=g) * 2 if kind != "equal" else torch.zeros(n)) + offset
+    f = lambda v: torch.full((B,), float(v))                                    # noqa: E731
+    i = lambda v: torch.full((B,), int(v), dtype=torch.int32)                   # noqa: E731
+    return dict(logits=x, u=f(u), inv_temp=f(filters.get("inv_temp", 1.0)), top_k=i(filters.get("top_k", 0)), top_p=f(filters.get("top_p", 1.0)),
+                min_p=f(filters.get("min_p", 0.0)), greedy=i(0))
+
+
+FILTERS_AT_ZERO = [{}, dict(top_k=50), dict(top_k=2000), dict(top_k=30000), dict(top_p=0.9), dict(top_p=0.9999999), dict(min_p=0.1), dict(min_p=1e-30), dict(top_k=4000, top_p=0.999),
+                   dict(top_k=40, min_p=1e-9), dict(top_p=0.99999, min_p=1e-20), dict(inv_temp=50.0), dict(inv_temp=50.0, top_k=3000)]
+
+
+def test_the_statement_draws_no_masked_token():
+    for low, offset in ((torch.finfo(torch.float32).min, 0.0), (-1e4, 1000.0), (-math.inf, 0.0), (-690.0, 12.0)):
+        for filters in FILTERS_AT_ZERO:
+            c = _masked_rows(300, low, offset, "short", 0.0, **filters)
+            tok, lp = SO.sample_filtered_ref(**c)
+            assert torch.all(c["logits"].gather(1, tok[:, None].long()) > low) and torch.all(lp > -700), (low, filters)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("low,offset", [(torch.finfo(torch.float32).min, 0.0), (-1e4, 0.0), (-690.0, 12.0), (torch.finfo(torch.float32).min, 1000.0), (-math.inf, 0.0)])
+@pytest.mark.parametrize("V", [37, 1024, 5000, 50001, 151936])
+def test_sampling_at_u_zero_takes_no_masked_token(V, low, offset):
+    for kind in ("short", "long", "equal"):
+        for filters in FILTERS_AT_ZERO:
+            for u in (0.0, 2.0 ** -24):
+                _check_sampling(_masked_rows(V, low, offset, kind, u, **filters))
+
+
 @pytest.mark.gpu
 def test_sampling_slices_streams_and_graphs():
     c = {k: v.cuda() for k, v in _sampling_case(33, 9973, 2, "peaked").items()}
