@@ -37,7 +37,7 @@ constexpr int SF_BINS = 2048;          // four for each thread
 constexpr int SF_CAP = 2048;           // entries of the list
 constexpr int SF_SEG = 256;            // logits of a piece of a block's share that has a sum of its own
 constexpr int SF_SEGS = 200;           // at most
-constexpr float SF_FAR = 16.6f;        // nats below the maximum from where single precision will do for a total (2^-24 of the maximum)
+constexpr float SF_FAR = 52.f;         // nats below the maximum from where tokens are left out of a total: 2^19 of them sum to less than 2^-56 of it
 constexpr int SF_LOADS = 10;           // 16-byte loads of a thread on their way: a share of 20480 logits at once
 constexpr int SF_GUESS = 256;          // tokens of a nucleus that is tried without a histogram of the row
 constexpr int SF_MAX_CLUSTER = 8;
@@ -595,8 +595,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     }
     if (guess) {
       const bool to_end = t_list == INFINITY, sums = by_mass && K == 0;
-      double s = 0.0, s_head = 0.0;
-      float far = 0.f;
+      double s = 0.0, s_head = 0.0;                        // (a list that does not go to the end is no deeper than the bins, 32 nats)
       int listed = 0;                                      // lane 31: entries of this warp
 #pragma unroll 2
       for (int i0 = 0; i0 < n4; i0 += SF_THREADS) {
@@ -611,27 +610,14 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
           some |= t[j] < t_list;
           near |= t[j] < SF_FAR * SF_PER_NAT;
         }
-        if (sums) {
-          if (near) {
-            double w[4];
+        if (sums && near) {
+          double w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = weight(fma((double)x[j], it, -top_it), sh.tab);
-            s += (w[0] + w[1]) + (w[2] + w[3]);
-            if (some) {
+          for (int j = 0; j < 4; ++j) w[j] = weight(fma((double)x[j], it, -top_it), sh.tab);
+          s += (w[0] + w[1]) + (w[2] + w[3]);
+          if (some) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) s_head += to_end || t[j] < t_list ? w[j] : 0.0;
-            }
-          } else {
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              f[j] = fast_exp2(t[j] * (-1.4426950408889634f / SF_PER_NAT));
-              far += f[j];
-            }
-            if (some) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) s_head += to_end || t[j] < t_list ? (double)f[j] : 0.0;
-            }
+            for (int j = 0; j < 4; ++j) s_head += to_end || t[j] < t_list ? w[j] : 0.0;
           }
         }
         if (__any_sync(0xffffffffu, some)) {
@@ -667,7 +653,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
         for (int i = tid; i < k && at + i < SF_CAP; i += SF_THREADS) head->list[at + i] = sh.list[i];
       }
       if (sums) {
-        s = warp_sum_d(s + (double)far);
+        s = warp_sum_d(s);
         s_head = warp_sum_d(s_head);
         if (lane == 0) { sh.red[warp] = s; sh.red2[warp] = s_head; }
       }
@@ -720,7 +706,6 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       // top-p needs fit between them.
       const bool sums = by_mass && K == 0 && !have_total;
       double q = 0.0;
-      float far = 0.f;
 #pragma unroll 2
       for (int i = tid; i < n4; i += SF_THREADS) {
         const float4 v = xs4[i];
@@ -733,19 +718,14 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
           near |= t[j] < SF_FAR * SF_PER_NAT;
           atomicAdd(&sh.hist[__float2uint_rz(fminf(t[j], (float)(SF_BINS - 1)))], 1u);
         }
-        if (sums) {
-          if (near) {
-            double w[4];
+        if (sums && near) {
+          double w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = weight(fma((double)x[j], it, -top_it), sh.tab);
-            q += (w[0] + w[1]) + (w[2] + w[3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) far += fast_exp2(t[j] * (-1.4426950408889634f / SF_PER_NAT));
-          }
+          for (int j = 0; j < 4; ++j) w[j] = weight(fma((double)x[j], it, -top_it), sh.tab);
+          q += (w[0] + w[1]) + (w[2] + w[3]);
         }
       }
-      if (sums) publish_sum(q + (double)far);
+      if (sums) publish_sum(q);
     }
     __syncthreads();
     {

@@ -734,6 +734,32 @@ def test_sampling_at_u_zero_takes_no_masked_token(V, low, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [131072, 151936, 393216])
+@pytest.mark.parametrize("first,at,end", [(16.61, 16.7, 16.85), (16.7, 18.0, 20.0), (30.0, 31.0, 33.0)])
+def test_sampling_of_nuclei_that_end_far_below_the_largest(V, first, at, end):
+    """One large logit and thousands of small ones, most of them ``first`` to ``at`` nats down and 6000 from there to ``end``, where the nucleus ends. Together they are a small part of the
+    total and each is 6e-8 of it or less: the border, and the token drawn next to the end of the sum, are those of a total in 64 bits, in
+    whatever order the tokens stand."""
+    g = torch.Generator().manual_seed(V)
+    it = torch.tensor([1 / 0.7]).float()
+    down = torch.cat([torch.linspace(first, at, V - 6001, dtype=torch.float64), torch.linspace(at, end, 6000, dtype=torch.float64)]).float() / it
+    x = torch.empty(16, V)
+    x[:, 0] = 195.0625 + 0.4375 * (torch.arange(16) % 8)                        # (times 64 / 0.7 it is rounded by nearly half a step of 32 bits, always upwards)
+    x[:, 1:] = x[:, :1] - down
+    w = torch.exp((x[0].double() - x[0, 0].double()) * it.double())
+    p = torch.tensor([float(w[:V - a].sum() / w.sum()) for a in (5000, 4000, 3000, 2500, 2000, 1500, 1000, 500)] * 2).clamp(max=1 - 2.0 ** -24).float()
+    for b in range(8, 16):
+        x[b] = x[b, torch.randperm(V, generator=g)]
+    c = dict(logits=x, u=torch.full((16,), 1 - 2.0 ** -24), inv_temp=it.expand(16).contiguous(), top_k=torch.zeros(16, dtype=torch.int32), top_p=p,
+             min_p=torch.zeros(16), greedy=None)
+    tok, lp = SO.sample_filtered_ref(**c)
+    got, glp = SO.sample_filtered(**{k: v if v is None else v.cuda() for k, v in c.items()})
+    assert torch.equal(got.cpu(), tok), (got.cpu() - tok).tolist()
+    assert torch.all((glp.cpu().double() - lp.double()).abs() <= 2.0 ** -23 * lp.abs().double() + 1e-9)
+    _no_kernel_error()
+
+
+@pytest.mark.gpu
 def test_sampling_slices_streams_and_graphs():
     c = {k: v.cuda() for k, v in _sampling_case(33, 9973, 2, "peaked").items()}
     first = SO.sample_filtered(**c)
