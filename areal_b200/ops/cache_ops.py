@@ -7,7 +7,8 @@ holds its largest finite element (|x| <= 448 * scale), never smaller than what t
 codes are rounded again to the new one. Writing slot 0 starts a page: what stood in it counts for nothing.
 
 As in :mod:`.functional`, CUDA tensors run the sm_100a kernels and CPU tensors the plain statements (``*_ref``), computed in 64 bits.
-The engine takes this cache with ``NativeInferConfig.kv_cache_dtype = "float8_e4m3"``.
+The engine takes this cache with ``NativeInferConfig.kv_cache_dtype = "float8_e4m3"``. There are no gradients: rows, queries or logits that require them are refused
+unless they are switched off.
 """
 from __future__ import annotations
 
@@ -51,6 +52,12 @@ class QuantPages:
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+def _no_gradients(*tensors) -> None:
+    """Refuses what a backward pass would expect a gradient for: the result would be cut off from it without a word."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("serving operators have no gradients: call them under torch.no_grad()")
 
 
 def _check_pages(p: QuantPages, dim: int, dev: int) -> tuple:
@@ -155,6 +162,7 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pages: QuantPages, page_table: 
     dev, (rows, Hkv, D) = k.get_device(), shape
     if v.get_device() != dev:
         raise ValueError("keys and values on different devices")
+    _no_gradients(k, v)
     P, heads, ps = _check_pages(pages, D, dev)
     if heads != Hkv:
         raise ValueError(f"rows of {Hkv} heads into a cache of {heads}")
@@ -232,6 +240,7 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     shape = q.shape
     if not (len(shape) == 3 and q.dtype is torch.bfloat16):
         raise ValueError("queries: bf16 [B, Hq, D]")
+    _no_gradients(q)
     dev, (B, Hq, D) = q.get_device(), shape
     P, Hkv, ps = _check_pages(pages, D, dev)
     width = _check_table(page_table, seq_lens, B, dev)

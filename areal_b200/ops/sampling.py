@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import lib as _lib
-from .cache_ops import _launch, _need
+from .cache_ops import _launch, _need, _no_gradients
 
 _V, _I, _L = _lib.c_void_p, _lib.c_int, _lib.c_ll
 NO_WEIGHT = -(700 + 2.0 ** -11)          # from here down a token has no weight: e^-700 is next to the smallest number of 64 bits
@@ -62,10 +62,11 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, inv_temp: torch.Tenso
     infinity and NaN have no weight, nor have those more than 700 nats below the largest; infinite ones share all of it. A row in which nothing has weight gives token -1 and minus infinity.
 
     ``u``, ``inv_temp``, ``top_p``, ``min_p``: fp32 ``[B]``; ``top_k``, ``greedy``: int32 ``[B]``. Rows of logits may lie apart (a slice of a wider
-    tensor). At most 393216 tokens in the vocabulary on CUDA."""
+    tensor). The log-prob has no gradient: logits that require one are refused unless gradients are switched off. At most 393216 tokens in the vocabulary on CUDA."""
     shape = logits.shape
     if not (len(shape) == 2 and logits.dtype is torch.float32 and shape[1] > 0 and (logits.stride(1) == 1 or shape[1] == 1)):
         raise ValueError("logits: fp32 [B, V], dense rows")
+    _no_gradients(logits, u, inv_temp, top_p, min_p)
     B, V = shape
     dev, one = logits.get_device(), shape[:1]
     for t, d, name in ((u, torch.float32, "u"), (inv_temp, torch.float32, "inv_temp"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"),

@@ -214,6 +214,23 @@ def test_sampling_refuses(what):
         SO.sample_filtered(**a)
 
 
+@pytest.mark.parametrize("which", ["k", "v", "q", "logits", "inv_temp"])
+def test_what_requires_a_gradient_is_refused_and_taken_without(which):
+    a = _append_args()
+    q, f, i = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.ones(3), torch.zeros(3, dtype=torch.int32)
+    s = dict(logits=torch.zeros(3, 10), u=f * 0.5, inv_temp=f.clone(), top_k=i, top_p=f, min_p=f * 0)
+    t, call = {"k": (a[0], lambda: CO.kv8_append(*a)), "v": (a[1], lambda: CO.kv8_append(*a)), "q": (q, lambda: CO.kv8_decode(q, *a[2:])),
+               "logits": (s["logits"], lambda: SO.sample_filtered(**s)), "inv_temp": (s["inv_temp"], lambda: SO.sample_filtered(**s))}[which]
+    call()
+    t.requires_grad_(True)
+    with pytest.raises(ValueError, match="no_grad"):
+        call()
+    with torch.no_grad():
+        call()
+    with torch.inference_mode():
+        call()
+
+
 def test_copies_on_the_host_leave_the_rest_of_a_page():
     t = torch.arange(2 * 5 * 4 * 3).view(2, 5, 4, 3).clone()
     s, was = torch.arange(10).view(2, 5).clone(), t.clone()
