@@ -155,7 +155,7 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pages: QuantPages, page_table: 
     sequence ``b`` brings the rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` as its last ones; rows behind ``cu_seqlens[B]`` are left out. Rows
     may be a part of a wider projection (``k.stride(0)`` a multiple of 8 elements, heads dense). A page that gets rows belongs to one
     sequence. ``page_table`` ``[B, width]`` int32; entries of a sequence beyond its length are not read. An entry out of the cache, or a
-    length beyond the table, sets the device error word (code 6) and writes nothing for that page."""
+    length beyond the table, sets the device error word (code 6) and writes nothing for that page (on the host: a ``ValueError``)."""
     shape = k.shape
     if not (len(shape) == 3 and v.shape == shape and k.dtype is torch.bfloat16 and v.dtype is torch.bfloat16):
         raise ValueError("keys and values: bf16 [rows, Hkv, D]")
@@ -198,7 +198,9 @@ def kv8_decode_ref(q, pages: QuantPages, page_table, seq_lens, scale: Optional[f
     for b, n in enumerate(seq_lens.tolist()):
         if n <= 0:
             continue
+        _need(n <= page_table.shape[1] * ps, f"sequence {b}: {n} tokens are more than its table holds")
         pg = page_table[b, :-(-n // ps)].long()
+        _need(bool(((pg >= 0) & (pg < pages.k.shape[0])).all()), f"a page of sequence {b} is not in the cache")
         K, V = ((c.view(torch.uint8)[pg].view(F8).double() * s[pg].double()[:, :, None, None]).transpose(0, 1).reshape(Hkv, -1, D)[:, :n]
                 for c, s in ((pages.k, pages.k_scale), (pages.v, pages.v_scale)))
         z = torch.einsum("hgd,htd->hgt", q[b].double().view(Hkv, Hq // Hkv, D), K) * scale
@@ -234,7 +236,7 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     ``q`` ``[B, Hq, D]`` bf16, heads dense, rows a multiple of 8 elements apart (the query part of a wider projection); ``Hq`` a multiple of the cache's
     heads, any number of query heads for each. ``scale`` defaults to ``1 / sqrt(D)``. Returns bf16 ``[B, Hq, D]`` (``out``, contiguous and apart from
     ``q``, where given); a sequence of length 0 gets zeros. Codes behind a sequence's last token may be anything. An entry of the table out of the cache, or a
-    length beyond the table, sets the device error word (code 6); the row's result is not to be used. The workspace
+    length beyond the table, sets the device error word (code 6); the row's result is not to be used (on the host: a ``ValueError``). The workspace
     belongs to the current stream or, in a captured call, to its graph: calls on several streams and graphs do not share one, and calls of several threads on
     one stream go one after the other. At most 8192 sequences."""
     shape = q.shape

@@ -123,6 +123,17 @@ def test_the_statement_refuses_pages_and_lengths_out_of_range(page, lens):
         CO.kv8_append(*a)
 
 
+@pytest.mark.parametrize("page,lens", [(4, 1), (-1, 1), (0, 33)])
+def test_decode_on_the_host_refuses_pages_and_lengths_out_of_range(page, lens):
+    _, _, p, table, n = _append_args()
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    table[1, 1], n[1] = -5, 16                                                  # an entry behind the sequence's length is not read
+    CO.kv8_decode(q, p, table, n)
+    table[1, 0], n[1] = page, lens
+    with pytest.raises(ValueError):
+        CO.kv8_decode(q, p, table, n)
+
+
 def test_decode_refuses_more_than_8192_sequences():
     p = CO.QuantPages.empty(1, 1, 16, 64, "cpu")
     for B in (8192, 8193):
