@@ -25,6 +25,7 @@ F8 = torch.float8_e4m3fn
 KV8_MAX = 448.0
 KV8_E_MIN, KV8_E_MAX = -100, 120
 PAGE_SIZES = (16, 32, 64, 128)
+WIDEST = (1 << 31) - 64                      # tokens of a page table: positions up to the end of a page or tile are counted in 32 bits
 
 _V, _I, _F, _L = _lib.c_void_p, _lib.c_int, _lib.c_float, _lib.c_ll
 
@@ -173,6 +174,8 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pages: QuantPages, page_table: 
         _need(B >= 0 and cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous() and cu_seqlens.get_device() == dev,
               "cu_seqlens: contiguous int32 [B + 1]")
     width = _check_table(page_table, seq_lens, B, dev)
+    if width * ps >= WIDEST:
+        raise ValueError("a table wider than 2^31 tokens")
     if dev < 0:
         return kv8_append_ref(k, v, pages, page_table, seq_lens, cu_seqlens)
     if rows == 0 or B == 0:
@@ -248,7 +251,7 @@ def kv8_decode(q: torch.Tensor, pages: QuantPages, page_table: torch.Tensor, seq
     width = _check_table(page_table, seq_lens, B, dev)
     if Hq <= 0 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads over {Hkv} cached ones")
-    if B > 8192 or width * ps >= (1 << 31) - 64:
+    if B > 8192 or width * ps >= WIDEST:
         raise ValueError("more than 8192 sequences, or a table wider than 2^31 tokens")
     if out is not None:
         _need(out.shape == shape and out.dtype == torch.bfloat16 and out.is_contiguous() and out.get_device() == dev, "out: contiguous bf16 like the queries")

@@ -16,6 +16,7 @@ extern "C" int ab2_num_sms();
 
 namespace ab2 {
 
+constexpr long long KV8_WIDEST = 0x7fffffffLL - 63;   // tokens of a table: the end of the last page or tile still is an int
 constexpr int KV8_E_MIN = -100, KV8_E_MAX = 120;       // exponents a scale may have; both its value and its inverse are normal
 
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
@@ -837,6 +838,7 @@ int ab2_kv8_append(const void* k, const void* v, void* kc, void* vc, void* ks, v
   if (D != 64 && D != 128) return 11;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return 12;
   if (Hkv <= 0 || Hkv > 4096 || (k_stride & 7) || (v_stride & 7) || width <= 0 || num_pages <= 0) return 10;
+  if ((long long)width * page_size >= KV8_WIDEST) return 13;
   int* err = ab2host::error_flag();
   Kv8Args a;
   a.x[0] = (const __nv_bfloat16*)k; a.x[1] = (const __nv_bfloat16*)v;
@@ -893,7 +895,7 @@ int ab2_kv8_decode(const void* q, const void* kc, const void* vc, const void* ks
   if (Hkv <= 0 || Hq % Hkv || (q_stride & 7) || width <= 0 || num_pages <= 0 || B > KV8_MOST_ROWS) return 10;
   const int G = Hq / Hkv, groups = (G + 15) / 16;
   // chunks of the whole batch are counted in 32 bits
-  if ((long long)width * page_size > 0x7fffffffLL - 64 || (long long)B * Hkv * groups * (((long long)width * page_size + 63) / 64) > 0x7fffffffLL - 65536) return 13;
+  if ((long long)width * page_size >= KV8_WIDEST || (long long)B * Hkv * groups * (((long long)width * page_size + 63) / 64) > 0x7fffffffLL - 65536) return 13;
   Kv8Decode a;
   const int grid = kv8_grid(B, Hq, Hkv, width, page_size, ab2_num_sms());
   a.q = (const __nv_bfloat16*)q; a.kc = (const unsigned char*)kc; a.vc = (const unsigned char*)vc;

@@ -134,6 +134,20 @@ def test_decode_on_the_host_refuses_pages_and_lengths_out_of_range(page, lens):
         CO.kv8_decode(q, p, table, n)
 
 
+@pytest.mark.parametrize("fits", [True, False])
+def test_tables_of_2_to_31_tokens_are_refused(fits):
+    """The end of a page has to be an int: 2^24 pages of 128 tokens are one too many."""
+    p = CO.QuantPages.empty(4, 2, 128, 64, "cpu")
+    k, q = torch.zeros(1, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    table, n = torch.zeros(1, 2 ** 24 - fits, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for call in (lambda: CO.kv8_append(k, k, p, table, n), lambda: CO.kv8_decode(q, p, table, n)):
+        if fits:
+            call()
+        else:
+            with pytest.raises(ValueError, match="2\\^31"):
+                call()
+
+
 def test_decode_refuses_more_than_8192_sequences():
     p = CO.QuantPages.empty(1, 1, 16, 64, "cpu")
     for B in (8192, 8193):
