@@ -359,6 +359,10 @@ def _ints(x) -> list:
 
 
 _lib.declare("ab2_kv8_append", [_V] * 9 + [_I] * 7 + [_L, _L, _V])
-_lib.declare("ab2_kv8_decode", [_V] * 9 + [_I] * 7 + [_F, _L, _V])
+def _decode_kernels(*a) -> int:
+    return 1 + (a[13] * a[14] > 4 * 64)          # the join, where the table holds more than the smallest unit's four chunks of 64 tokens
+
+
+_lib.declare("ab2_kv8_decode", [_V] * 9 + [_I] * 7 + [_F, _L, _V], kernels=_decode_kernels)
 _lib.declare("ab2_kv8_decode_workspace", [_I] * 6, _L)
-_lib.declare("ab2_copy_pages", [_V, _I, _V, _I, _V])
+_lib.declare("ab2_copy_pages", [_V, _I, _V, _I, _V], kernels=lambda *a: -(-a[3] // 256))           # pairs travel 256 at a time

@@ -123,8 +123,8 @@ def get_lib():
     return _LIB
 
 
-# Number of kernels each exported launcher enqueues (used for launch accounting).
-_KERNELS_PER_CALL = {"ab2_kernel_error_peek": 0, "ab2_gemm_splitk": 2, "ab2_paged_decode": 2, "ab2_paged_decode_strided": 2, "ab2_paged_decode_noalloc": 2, "ab2_kv8_decode": 2, "ab2_kv8_decode_workspace": 0, "ab2_kernel_error": 0, "ab2_runtime_init": 0, "ab2_num_sms": 0}
+# Number of kernels each exported launcher enqueues (used for launch accounting): one where nothing is said, or a function of the call's arguments.
+_KERNELS_PER_CALL = {"ab2_kernel_error_peek": 0, "ab2_gemm_splitk": 2, "ab2_paged_decode": 2, "ab2_paged_decode_strided": 2, "ab2_paged_decode_noalloc": 2, "ab2_kv8_decode_workspace": 0, "ab2_kernel_error": 0, "ab2_runtime_init": 0, "ab2_num_sms": 0}
 LAUNCHES = {"count": 0}
 
 
@@ -145,9 +145,14 @@ class _CountingLib:
             c[name] = fn
             return fn
 
-        def call(*a, _fn=fn, _n=n):
-            LAUNCHES["count"] += _n
-            return _fn(*a)
+        if callable(n):
+            def call(*a, _fn=fn, _n=n):
+                LAUNCHES["count"] += _n(*a)
+                return _fn(*a)
+        else:
+            def call(*a, _fn=fn, _n=n):
+                LAUNCHES["count"] += _n
+                return _fn(*a)
         c[name] = call
         return call
 
@@ -156,9 +161,12 @@ def launch_count() -> int:
     return LAUNCHES["count"]
 
 
-def declare(name: str, argtypes, restype=c_int) -> None:
-    """Registers the signature of an additional exported symbol."""
+def declare(name: str, argtypes, restype=c_int, kernels=None) -> None:
+    """Registers the signature of an additional exported symbol, and the kernels that a call enqueues where that is not one (a number, or a function of
+    the call's arguments)."""
     _SIGS[name] = (argtypes, restype)
+    if kernels is not None:
+        _KERNELS_PER_CALL[name] = kernels
     if _LIB is not None and hasattr(_LIB._lib, name):
         fn = getattr(_LIB._lib, name)
         fn.argtypes, fn.restype = argtypes, restype

@@ -624,6 +624,44 @@ def test_decode_called_by_threads_that_share_a_stream():
     _no_kernel_error()
 
 
+# ----------------------------------------------------------------------------- launch accounting
+def test_kernels_of_a_call_are_counted_from_its_arguments(monkeypatch):
+    class Fake:
+        def __getattr__(self, name):
+            return lambda *a: 0
+    fake = oplib._CountingLib(Fake())
+
+    def counted(name, *a):
+        before = oplib.launch_count()
+        getattr(fake, name)(*a)
+        return oplib.launch_count() - before
+    monkeypatch.setitem(oplib.LAUNCHES, "count", 0)
+    decode = lambda ps, width: counted("ab2_kv8_decode", *[0] * 9, 3, 8, 2, 64, ps, width, 10, 1.0, 0, 0)      # noqa: E731
+    assert [decode(64, 4), decode(64, 5), decode(16, 16), decode(16, 17), decode(128, 2), decode(128, 3)] == [1, 2, 1, 2, 1, 2]
+    assert [counted("ab2_copy_pages", b"", 1, b"", n, 0) for n in (1, 256, 257, 1000)] == [1, 1, 2, 4]
+    assert counted("ab2_kv8_append") == 1 and counted("ab2_sample_filtered") == 1 and counted("ab2_gemm_splitk") == 2 and counted("ab2_num_sms") == 0
+
+
+@pytest.mark.gpu
+def test_kernels_counted_are_those_of_a_captured_call():
+    from cuda.bindings import runtime as rt
+
+    t, s = torch.zeros(700, 16, 8, device="cuda"), torch.cuda.Stream()
+    small, long = (tuple(x.cuda() if torch.is_tensor(x) else _clone(x, "cuda") for x in _decode_case(2, 8, 2, 64, 16, lens, 8, width=w)) for lens, w in (([200, 5], 16), ([250, 5], 17)))
+    c = {k: v.cuda() for k, v in _sampling_case(3, 1000, 1, "normal").items()}
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    for call, n in ((lambda: CO.kv8_decode(*small), 1), (lambda: CO.kv8_decode(*long), 2), (lambda: CO.copy_pages([(t, 0, 1)], range(300), range(300, 600)), 2),
+                    (lambda: CO.copy_pages([(t, 0, 1)], [0], [1]), 1), (lambda: CO.kv8_append(k, k, small[1], small[2], small[3]), 1), (lambda: SO.sample_filtered(**c), 1)):
+        call()
+        torch.cuda.synchronize()
+        g, before = torch.cuda.CUDAGraph(keep_graph=True), oplib.launch_count()
+        with torch.cuda.graph(g, stream=s):
+            call()
+        assert oplib.launch_count() - before == n
+        err, _, nodes = rt.cudaGraphGetNodes(rt.cudaGraph_t(g.raw_cuda_graph()), 0)
+        assert int(err) == 0 and nodes == n
+
+
 # ----------------------------------------------------------------------------- page copies
 @pytest.mark.gpu
 @pytest.mark.parametrize("Hkv,D,ps,layers", [(8, 128, 64, 3), (2, 64, 16, 4), (1, 128, 128, 1), (3, 24, 20, 2)])
