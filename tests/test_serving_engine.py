@@ -201,6 +201,41 @@ def test_device_and_host_filters_leave_the_same_distribution():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_filters_on_the_device_serve_a_mixer_stack(monkeypatch, dtype):
+    """Requests of a mixer stack with filters, without and greedy, side by side: every draw is the statement's on the step's own logits, with the numbers that
+    belong to the requests' seeds and positions, and the tokens are those drawn; top-k 1 and greedy agree."""
+    model = build_model(preset("tiny-kagolix"), dtype=dtype, device="cuda", seed=7)
+    e = _engine(model, filtered_sampling="device")
+    calls, inner = [], IE.OS.sample_filtered
+
+    def watched(*a, **kw):
+        calls.append([x.clone() for x in a])
+        r = inner(*a, **kw)
+        calls[-1].append([x.clone() for x in r])
+        return r
+    monkeypatch.setattr(IE.OS, "sample_filtered", watched)
+    kinds = [dict(top_k=5), dict(top_p=0.8, temperature=0.7), {}, dict(greedy=True), dict(min_p=0.1, top_k=40), dict(top_k=1), dict(top_p=0.95, top_k=9, seed=77)]
+    prompts = [list(range(3, 40))] * len(kinds)
+
+    async def go():
+        return await asyncio.gather(*[e.agenerate(ModelRequest(rid=f"r{i}", input_ids=p, gconfig=GenerationHyperparameters(
+            **{"max_new_tokens": 20, "max_tokens": 400, "ignore_eos": True, **k}))) for i, (p, k) in enumerate(zip(prompts, kinds))])
+    rs = asyncio.run(go())
+    e.destroy()
+    assert oplib.kernel_error() == 0
+    assert rs[3].output_tokens == rs[5].output_tokens and max(abs(x) for x in rs[5].output_logprobs) == 0
+    assert sum(c[0].shape[0] for c in calls) >= 20 * sum(bool(k) and k != dict(greedy=True) for k in kinds)
+    drawn = set()
+    for *a, (tok, lp) in calls:
+        want, wlp = IE.OS.sample_filtered_ref(*(x.cpu() for x in a))
+        assert torch.equal(tok.cpu(), want) and torch.all((lp.cpu().double() - wlp.double()).abs() <= 2.0 ** -23 * wlp.abs().double() + 1e-9)
+        drawn |= {(float(u), int(t), float(p)) for u, t, p in zip(a[1].cpu(), tok.cpu(), lp.cpu())}
+    for n, (tok, lp) in enumerate(zip(rs[6].output_tokens, rs[6].output_logprobs)):
+        assert (IE._uniform01(77, len(prompts[6]) + n), tok, lp) in drawn
+
+
+@pytest.mark.gpu
 def test_a_cache_the_kernels_do_not_take_is_refused():
     model = build_model(preset("tiny-qwen3"), dtype=torch.bfloat16, device="cuda", seed=5)
     with pytest.raises(ValueError):
