@@ -502,13 +502,14 @@ class NativeInferConfig:
     # KV pool in pausable memory (addresses survive while the physical pages leave the GPU): offload() then
     # really returns the pool's memory to the device and onload() takes it back without re-capturing CUDA graphs
     pausable_kv_cache: bool = False
-    # bfloat16, or float8_e4m3 (also fp8_e4m3): codes with a power-of-two scale for each page and head, half the bytes per decode step and
-    # twice the tokens in the pool; head sizes 64 and 128, models on the paged cache
-    kv_cache_dtype: str = "bfloat16"
+    # In 8 bits codes with a power-of-two scale for each page and head, for models on the paged cache. A file that set fp8_e4m3 or fp8 before the key
+    # was read now gets an 8-bit cache, and an error with heads or pages that it does not take.
+    kv_cache_dtype: str = "bfloat16"  # bfloat16, or float8_e4m3 (also fp8_e4m3, fp8): half the cache bytes, codes of four significant bits; heads of 64 or 128, pages of 16, 32, 64 or 128 tokens
     # Requests with top-k / top-p / min-p: "host" copies the step's logits and sorts them there, row by row (the draws of earlier versions);
     # "device" samples them in one kernel, with draws of its own that depend on the request's seed and the position (stacks of the
-    # gated delta rule sample on the host either way)
-    filtered_sampling: str = "host"
+    # gated delta rule sample on the host either way). Of tokens that tie with the last of a top-k the host keeps all, the device the
+    # lowest indices up to k; LM-head products are rounded to 16 bits, so ties are not rare.
+    filtered_sampling: str = "host"  # where top-k / top-p / min-p are applied: host, or device (one kernel, draws of its own; exactly k tokens of a top-k, where the host keeps all that tie with the last)
     use_cuda_graph: bool = True
     compute_dtype: str = "bfloat16"  # float32: matrices, activations and cache in 32 bits (mixer stacks only)
     weight_dtype: str = "bfloat16"  # or float8_e4m3fn (block-scaled)

@@ -119,6 +119,13 @@ def test_example_configs_parse_and_backend_extras_are_kept():
     assert cfg.actor.use_kernels is False and cfg.rollout.poll_interval == 0.1
 
 
+def test_config_reference_says_what_the_serving_options_mean():
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "docs", "config_reference.md")).read()
+    for key, words in (("kv_cache_dtype", ("float8_e4m3", "fp8", "pages of 16")), ("filtered_sampling", ("host", "device", "exactly k")), ("min_p", ("likeliest",))):
+        line = next(x for x in text.splitlines() if x.startswith(f"| `{key}` |"))
+        assert all(w in line for w in words), line
+
+
 def test_config_reference_is_generated_from_the_dataclasses():
     from areal_b200.tools import generate_cli_docs as G
 

@@ -51,6 +51,28 @@ def test_min_p_travels_with_a_request_and_filters_on_the_host():
     e.destroy()
 
 
+def test_tokens_that_tie_with_the_last_of_a_top_k():
+    """The host keeps them all, the device the lowest indices up to k: log-probs differ by the tokens more, and agree where nothing ties."""
+    model = build_model(preset("tiny-qwen3"), dtype=torch.float32, device="cpu", seed=3)
+    e = _engine(model, "cpu")
+    s = IE._Seq(rid="a", tokens=[1], prompt_len=1, max_new=1, min_new=0, temperature=1.0, greedy=False, stop_ids=set(), ignore_eos=True, seed=1, top_k=3)
+    for logits, host, device in ((torch.tensor([1.0, 2.0, 3.0, 2.0, 2.0, -1.0]), {1, 2, 3, 4}, {1, 2, 3}), (torch.tensor([1.0, 2.5, 3.0, 2.0, 1.5, -1.0]), {1, 2, 3}, {1, 2, 3})):
+        seen = {}
+        for n in range(200):
+            s.tokens = [1] * (n + 1)
+            tok, lp = e._sample_cpu(logits, s)
+            seen[tok] = lp
+        assert set(seen) == host
+        u = (torch.arange(200) + 0.5) / 200
+        one = torch.ones(200)
+        tok, lp = IE.OS.sample_filtered(logits.expand(200, 6).contiguous(), u, one, (one * 3).int(), one, one * 0)
+        assert set(tok.tolist()) == device
+        for kept, got in ((host, seen), (device, dict(zip(tok.tolist(), lp.tolist())))):
+            want = torch.log_softmax(logits[sorted(kept)], 0)
+            assert max(abs(got[t] - float(want[i])) for i, t in enumerate(sorted(kept))) < 1e-6
+    e.destroy()
+
+
 def test_unknown_sampling_places_are_refused():
     with pytest.raises(ValueError):
         NativeInferenceEngine(InferenceEngineConfig(), NativeInferConfig(filtered_sampling="gpu"), model_config=preset("tiny-qwen3"))
