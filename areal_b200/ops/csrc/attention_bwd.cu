@@ -207,7 +207,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const size_t vec_idx = (size_t)hq * T + seq_start + q_local;
       const float lse2 = q_valid ? LSE[vec_idx] * 1.4426950408889634f : 0.f;
       const float dlt = q_valid ? DELTA[vec_idx] : 0.f;
-      if (!mbar_wait(s_full, ph, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
+      if (!mbar_wait_warp(s_full, ph, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
       tc_fence_after();
       const bool diag = causal && (i == jb);
       const bool tail = (jb * BKV + BKV > seq_len);
@@ -245,7 +245,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       tc_fence_before();
       mbar_arrive(pds_ready);
       // dQ block -> global fp32 accumulation
-      if (!mbar_wait(dq_full, ph, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
+      if (!mbar_wait_warp(dq_full, ph, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
       tc_fence_after();
       float* dq_row = dQ + ((size_t)(seq_start + q_local) * Hq + hq) * HD;
 #pragma unroll 1

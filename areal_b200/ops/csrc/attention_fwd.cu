@@ -178,7 +178,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     for (int j = 0; j < nkv && ok; ++j) {
       const int sb = j & 1;
       const uint32_t ph = static_cast<uint32_t>(j >> 1) & 1u;
-      if (!mbar_wait(s_full(sb), ph, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
+      if (!mbar_wait_warp(s_full(sb), ph, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
       tc_fence_after();
       const uint32_t t_s = tmem_base + lane_off + (sb ? Cfg::S_COL1 : Cfg::S_COL0);
       const int kv0 = j * KT;
@@ -205,7 +205,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const float alpha = (m_run == -INFINITY) ? 0.f : fast_exp2(m_run - m_use);
       // P smem (and O) may only be touched once the previous PV has retired.
       if (j > 0) {
-        if (!mbar_wait(o_ready, static_cast<uint32_t>(j - 1) & 1u, err, ERR_WAIT_MISC)) { ok = false; break; }
+        if (!mbar_wait_warp(o_ready, static_cast<uint32_t>(j - 1) & 1u, err, ERR_WAIT_MISC)) { ok = false; break; }
         tc_fence_after();
       }
       // pass 2: probabilities -> bf16 P in swizzled smem, row sum
@@ -264,7 +264,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
     // ---- epilogue: O / l -> global, log-sum-exp
     if (ok && nkv > 0) {
-      if (mbar_wait(o_ready, static_cast<uint32_t>(nkv - 1) & 1u, err, ERR_WAIT_MISC)) {
+      if (mbar_wait_warp(o_ready, static_cast<uint32_t>(nkv - 1) & 1u, err, ERR_WAIT_MISC)) {
         tc_fence_after();
         const bool valid = q_local < seq_len;
         const float inv_l = l_run > 0.f ? 1.f / l_run : 0.f;

@@ -103,6 +103,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* fl
   return true;
 }
 
+// The same for a whole warp: its lanes give up together. The instructions behind such a wait (tcgen05.ld, votes, shuffles) need all of them,
+// and a barrier that completes just as the limit runs out would otherwise let some lanes on and not the others.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int* flag, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, flag, code));
+}
+
 // ---------------------------------------------------------------- TMA
 // 2-D tiled load global -> shared of one box, completion counted on an mbarrier.
 // Never multicast: each CTA fetches its own tiles.

@@ -221,7 +221,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const int buf = local & 1;
       const uint32_t use = static_cast<uint32_t>(local >> 1);
       void* Cptr_t = SPLITK ? static_cast<void*>(reinterpret_cast<float*>(Cptr) + (size_t)(tile / mn_tiles) * M * ldc) : Cptr;
-      ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(buf), use & 1u, err, ERR_WAIT_TMEM_FULL));   // the warp leaves together
+      ok = mbar_wait_warp(tfull_bar(buf), use & 1u, err, ERR_WAIT_TMEM_FULL);   // the warp leaves together
       if (!ok) break;
       tc_fence_after();
       const int row = m0 + row_in_tile;

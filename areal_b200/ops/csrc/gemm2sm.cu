@@ -240,7 +240,7 @@ gemm_bf16_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const int m0 = mp * 2 * P2_BM + (int)crank * P2_BM, n0 = nb * P2_BN;
       const int buf = local & 1;
       const uint32_t use = static_cast<uint32_t>(local >> 1);
-      ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(buf), use & 1u, err, ERR_WAIT_TMEM_FULL));
+      ok = mbar_wait_warp(tfull_bar(buf), use & 1u, err, ERR_WAIT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
       const int row = m0 + row_in_tile;

@@ -170,7 +170,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         for (int kb = 0; kb < num_kb; ++kb, ++nbuf) {
           const int buf = (int)(nbuf & 1u);
           const float s = (row_ok ? sa[(size_t)kb * M + row] : 0.f) * sb[(size_t)nb * num_kb + kb];
-          if (!mbar_wait(tfull_bar(buf), (nbuf >> 1) & 1u, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
+          if (!mbar_wait_warp(tfull_bar(buf), (nbuf >> 1) & 1u, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * F8_BN;
 #pragma unroll
@@ -211,7 +211,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
       } else {
         const int buf = (int)(nbuf & 1u);
-        if (!mbar_wait(tfull_bar(buf), (nbuf >> 1) & 1u, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
+        if (!mbar_wait_warp(tfull_bar(buf), (nbuf >> 1) & 1u, err, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
         tc_fence_after();
         const float sr = row_ok ? sa[row] : 0.f;
         const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * F8_BN;

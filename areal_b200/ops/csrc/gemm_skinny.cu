@@ -136,7 +136,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     // epilogue: thread <-> one output feature (TMEM lane), loop over token columns
     const int q = warp & 3;
     const int n = n0 + q * 32 + lane;
-    if (mbar_wait(tfull_bar, 0u, err, ERR_WAIT_TMEM_FULL)) {
+    if (mbar_wait_warp(tfull_bar, 0u, err, ERR_WAIT_TMEM_FULL)) {
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1

@@ -641,7 +641,7 @@ chunk_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         for (int x = lane; x < 95; x += 32) bs[x] = r1 * __log2f(1.f + r2 * (float)max(first + qd * 32 - kb + x - 63, 0));
         __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, j & 1), (uint32_t)(j >> 1) & 1u, err, ERR_WAIT_TMEM_FULL));
+      ok = mbar_wait_warp(s_full(t, j & 1), (uint32_t)(j >> 1) & 1u, err, ERR_WAIT_TMEM_FULL);
       if (!ok) break;                                          // a warp gives up as a whole
       tc_fence_after();
       uint32_t u[64];
@@ -687,7 +687,7 @@ chunk_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       l_run = l_run * alpha + sum;
       tmem_st32(s_col(t, j & 1) + lane_off, pk);
       if (j > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (uint32_t)(j - 1) & 1u, err, ERR_WAIT_MISC));
+        ok = mbar_wait_warp(o_done(t), (uint32_t)(j - 1) & 1u, err, ERR_WAIT_MISC);
         if (!ok) break;
         tc_fence_after();
         if (any_grow) {
@@ -706,7 +706,7 @@ chunk_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tc_fence_before();
       mbar_arrive(p_ready(t));
     }
-    if (ok && nbt > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (uint32_t)(nbt - 1) & 1u, err, ERR_WAIT_MISC));
+    if (ok && nbt > 0) ok = mbar_wait_warp(o_done(t), (uint32_t)(nbt - 1) & 1u, err, ERR_WAIT_MISC);
     if (ok && nbt > 0) {
       tc_fence_after();
       float inv = l_run > 0.f ? p.x.out_scale / l_run : 0.f;

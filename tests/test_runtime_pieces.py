@@ -261,3 +261,23 @@ def test_small_config_switches_take_effect(tmp_path):
     eng.pause_generation()
     assert time.time() - t0 >= 0.3
     eng.continue_generation()
+
+
+def test_warps_give_up_a_wait_together():
+    """Waits of whole warps for an accumulator or an output, in front of instructions that need all lanes (tcgen05.ld), end for all lanes alike. The waits of one
+    elected lane may end as they like."""
+    import re
+    from pathlib import Path
+
+    import areal_b200.ops as ops
+
+    seen = 0
+    for f in sorted((Path(ops.__file__).parent / "csrc").glob("*.cu")):
+        text = f.read_text()
+        if "tmem_ld" not in text:
+            continue
+        for name, bar in re.findall(r"\b(mbar_wait\w*)\(((?:tfull_bar|s_full|dq_full|o_ready|o_done)\b[^;]*?), err, ERR_WAIT_(?:TMEM_FULL|MISC)\)", text):
+            elected = f.name == "mixer_attention.cu" and bar == "o_done(t), (uint32_t)j & 1u"        # the lane that issues the products
+            assert elected or name == "mbar_wait_warp", (f.name, bar)
+            seen += not elected
+    assert seen >= 14
