@@ -196,14 +196,30 @@ def run_mixer_serve(design):
     return 0
 
 
+def start_watchdog(seconds: float, progress, detail, gap: float = 4.0) -> None:
+    """A process that still runs after ``seconds`` prints every thread's stack to stderr, then what ``progress()`` says, at once and ``gap`` seconds later (the same: the run
+    stands; more: it is slow), then ``detail()``, which may wait for a lock, and ends. Where no Python code can run any more a signal ends it a
+    little later."""
+    import faulthandler
+    import signal
+
+    def report():
+        time.sleep(seconds + 0.5)
+        for wait, say in ((0.0, progress), (gap, progress), (0.0, detail)):
+            time.sleep(wait)
+            print(f"watchdog: {say()}", file=sys.stderr, flush=True)
+        os._exit(1)
+    faulthandler.dump_traceback_later(seconds, exit=False)
+    signal.setitimer(signal.ITIMER_REAL, seconds + gap + 6.0)
+    threading.Thread(target=report, name="watchdog", daemon=True).start()
+
+
 def main():
     args = parse_args()
     if args.impl == "reference":
         return run_reference(args)
     if args.workload == "mixer-serve":
         return run_mixer_serve(args.design)
-    import faulthandler
-
     # decode-path switches of the kernel library, read once per process at first use: programmatic
     # dependent launch between the kernels of a captured decode step and split-K for the
     # decode-sized projections (measured +4.7% tokens/s on one GPU with both on)
@@ -226,7 +242,13 @@ def main():
     # (default: shortly before the 870 s a benchmark run is given, so that a stall leaves stacks behind, not just a kill)
     wd = float(os.environ.get("AREAL_BENCH_WATCHDOG_S", "850") or 0)
     if wd > 0:
-        faulthandler.dump_traceback_later(wd, exit=True)
+        from areal_b200.ops import lib as oplib
+
+        def memory():
+            m = torch.cuda.memory_stats() if torch.cuda.is_initialized() else {}
+            return (f"allocator retries {m.get('num_alloc_retries', 0)}, reserved {m.get('reserved_bytes.all.current', 0) / 2 ** 30:.1f} GB, "
+                    f"allocated {m.get('allocated_bytes.all.current', 0) / 2 ** 30:.1f} GB")
+        start_watchdog(wd, lambda: f"kernel launches so far {oplib.launch_count()}", memory)
 
     try:
         result = run_async_grpo_bench(args, ClockSampler)

@@ -281,3 +281,21 @@ def test_warps_give_up_a_wait_together():
             assert elected or name == "mbar_wait_warp", (f.name, bar)
             seen += not elected
     assert seen >= 14
+
+
+@pytest.mark.parametrize("blocked", ["detail", "nothing"])
+def test_a_benchmark_that_does_not_end_says_whether_it_stands(blocked):
+    """Stacks, the count twice, the rest, and an exit code; where the rest never comes, a signal."""
+    code = f"""
+import sys, time
+sys.path.insert(0, {os.path.dirname(os.path.dirname(os.path.abspath(__file__)))!r})
+import bench
+t0 = time.time()
+bench.start_watchdog(0.5, lambda: f"count {{int(10 * (time.time() - t0))}}", (lambda: time.sleep(60)) if {blocked == "detail"} else (lambda: "memory"), gap=0.5)
+time.sleep(60)
+"""
+    t0 = time.time()
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=50)
+    lines = [x for x in r.stderr.splitlines() if x.startswith("watchdog:")]
+    assert "most recent call first" in r.stderr and lines[0].startswith("watchdog: count ") and lines[0] != lines[1] and time.time() - t0 < 40
+    assert (r.returncode == 1 and lines[2:] == ["watchdog: memory"]) if blocked == "nothing" else (r.returncode == -14 and len(lines) == 2)
