@@ -230,8 +230,8 @@ kv8_append_page_kernel(const __grid_constant__ Kv8Args a, const int* __restrict_
 // P is rounded to fp16 (half a step 2^-11) and multiplies codes, so it holds the page's value scale: probability times scale, what the token can add to
 // the result, as 2^(x + log2 scale - d). The largest of it seen lies between 2^8 and 2^15 (m and d only move when a token leaves that range), so that all
 // down to 2^-22 of the largest keep all bits, whatever the scales are and in whatever order the pages come. The sum of the probabilities
-// alone has a reference of its own, m: a token may have all the weight and add next to nothing, or the other way round. m and d are whole
-// numbers, d counted from m: moving them multiplies by powers of two, and neither rounds where scores are large.
+// alone has a reference of its own, m: a token may have all the weight and add next to nothing, or the other way round. d is counted from m, so
+// that it stays within a few hundred and is not rounded where scores are large.
 constexpr int KV8_CHUNK = 64, KV8_MOST_ROWS = 8192;
 constexpr int KV8_LEAST = 4;        // chunks of the smallest unit: what a split saves of so short an item, the join costs
 constexpr float KV8_LOW = -300.f;   // below every d: a scale is 2^-100 or more
@@ -281,7 +281,7 @@ __device__ __forceinline__ float log2_scale(float s) {
   if (s > 0.f) return bits & 0x7fffff ? e + __log2f(__int_as_float((bits & 0x7fffff) | 0x3f800000)) : e;
   return s == 0.f ? -INFINITY : NAN;
 }
-// a * 2^d in two steps: 2^d alone may be out of range where the product is not.
+// a * 2^d, d whole, in two steps: 2^d alone may be out of range where the product is not.
 __device__ __forceinline__ float times_pow2(float a, float d) {
   const int k = (int)fminf(fmaxf(d, -250.f), 250.f), h = k >> 1;
   return a * pow2i(h) * pow2i(k - h);
@@ -577,9 +577,9 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float m = fmaxf(m_run[t][e], ceilf(top) - 9.f);                       // the largest probability becomes 2^8 to 2^9
+            const float m = fmaxf(m_run[t][e], top - 9.f);                              // the largest probability becomes 2^9, which fp16 holds exactly
             const float d_old = d_run[t][e] - (m - m_run[t][e]);                        // the same unit of the sums, counted from the new m
-            const float d = fmaxf(fmaxf(d_old, ceilf(top - m + lv) - 9.f), KV8_LOW);    // and the largest share of the result too
+            const float d = fmaxf(fmaxf(d_old, ceilf(top - m + lv) - 9.f), KV8_LOW);    // and the largest share of the result 2^8 to 2^9
             if (m > m_run[t][e]) {
               l_run[t][e] *= fast_exp2(m_run[t][e] - m);
               m_run[t][e] = m;
@@ -653,6 +653,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8Decode a) {
       float dx = mm[g] - mx + md[g];                            // the warps' units, counted from the largest m
 #pragma unroll
       for (int w = 1; w < 4; ++w) dx = fmaxf(dx, mm[w * HP + g] - mx + md[w * HP + g]);
+      dx = ceilf(dx);                                           // (whole, for times_pow2)
       float l = 0.f, acc = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -730,6 +731,7 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const __grid_constant__ K
       f[w] = sm[w] - mx + sd[w];
       dx = fmaxf(dx, f[w]);
     }
+    dx = ceilf(dx);
 #pragma unroll
     for (int w = 0; w < 4; ++w) f[w] = fast_exp2(f[w] - dx);
     for (int d = threadIdx.x; d < D; d += 128)

@@ -503,6 +503,25 @@ def test_decode_of_pages_whose_value_scales_are_far_apart(Hq, Hkv, D, ps, n, apa
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [40, 250])
+def test_decode_where_one_token_has_most_of_the_weight(n):
+    """The largest probability is a power of two in fp16's unit and not rounded, so that the rounding of the others is all there is: less than a tenth of the weight on average, off by 2^-11 of itself at
+    most. A result is on the other side of a border of bf16, whose steps are 2^-8 of it or more, with a probability of 0.1 * 2^-11 / 2^-9 = 2.5 % at most."""
+    q, p, table, lens = _decode_case(64, 32, 8, 128, 64, [n] * 64, n)
+    p.k.copy_((torch.randn(p.k.shape, generator=torch.Generator().manual_seed(n)) * 0.02).to(F8))              # scores of a few tenths, and one of ln(9 n) or a little more
+    p.k_scale.fill_(1.0)
+    p.v_scale.fill_(1.0)
+    q[..., 0] = 1.0
+    for b in range(64):
+        at = (37 * b) % n
+        p.k.view(torch.uint8)[table[b, at // 64].long(), :, at % 64, 0] = torch.tensor([math.log(9 * n) * 1.1]).to(F8).view(torch.uint8)
+    ref = CO.kv8_decode_ref(q, p, table, lens, 1.0)
+    out = CO.kv8_decode(q.cuda(), _clone(p, "cuda"), table.cuda(), lens.cuda(), 1.0).cpu()
+    _no_kernel_error()
+    assert float((out != ref.to(torch.bfloat16)).double().mean()) < 0.025
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 200, 6000])
 def test_decode_of_the_largest_and_smallest_values(n):
     """Values next to bf16's largest number and to a scale's smallest: the result lies among them and is a number."""
