@@ -742,7 +742,6 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     }
     int c_total;
     const int c_before = block_scan_i((int)(c[0] + c[1] + c[2] + c[3]), sh.ired, &c_total);
-    K = min(K, c_total);                                                          // no more tokens than that have any weight
     do {
       if (tid == 0) { sh.cut[0] = SF_BINS; sh.cut[1] = SF_BINS; sh.cut[2] = c_total; sh.cut[3] = 0; }
       __syncthreads();
