@@ -94,9 +94,9 @@ __device__ __forceinline__ double weight(double d, const double* tab) {
   const bool gone = (unsigned int)__double2hiint(d) > 0xc085e000u;
   return __hiloint2double(gone ? 0 : __double2hiint(w) + ((k >> 5) << 20), __double2loint(w));
 }
-// Order-preserving map of floats to unsigned.
+// Order-preserving map of floats to unsigned; the two zeros are one value.
 __device__ __forceinline__ unsigned int key_of(float x) {
-  const unsigned int b = __float_as_uint(x);
+  const unsigned int b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float float_of(unsigned int k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }

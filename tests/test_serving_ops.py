@@ -859,6 +859,22 @@ def test_sampling_of_nuclei_that_end_far_below_the_largest(V, first, at, end):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 37, 1024, 5000, 50001])
+def test_sampling_takes_both_zeros_for_one_value(V):
+    """Logits of plus and minus zero tie, as the largest value, at the end of a top-k and at the border of a nucleus: the lowest indices come first."""
+    g = torch.Generator().manual_seed(V)
+    B = 24
+    for top in (0.0, 3.0):
+        x = (torch.randn(B, V, generator=g) * 1.2 + top / 2).round().clamp(max=top)
+        x = torch.where(x == 0, torch.where(torch.rand(B, V, generator=g) < 0.5, 0.0, -0.0), x)
+        above = (x > 0).sum(1)
+        for filters in (dict(top_k=above + 1), dict(top_k=above + V // 8 + 1), dict(top_p=0.0), dict(top_p=0.5), dict(top_p=0.7, top_k=torch.full((B,), V - 1)), dict(top_k=above + 3, top_p=0.6)):
+            p = filters.get("top_p", 1.0)
+            _check_sampling(dict(logits=x, u=torch.rand(B, generator=g), inv_temp=torch.ones(B), top_k=filters.get("top_k", torch.zeros(B)).int(), top_p=torch.full((B,), p),
+                                 min_p=torch.zeros(B), greedy=(torch.arange(B) % 6 == 5).int()))
+
+
+@pytest.mark.gpu
 def test_sampling_slices_streams_and_graphs():
     c = {k: v.cuda() for k, v in _sampling_case(33, 9973, 2, "peaked").items()}
     first = SO.sample_filtered(**c)
