@@ -213,7 +213,7 @@ kv8_append_page_kernel(const __grid_constant__ Kv8Args a, const int* __restrict_
 
 // ------------------------------------------------------------------ attention of single tokens
 // o = softmax(scale * q K^T) V over the first lens[b] tokens, G query heads for each key/value head. Bound by the codes' bytes: 256 x 2000..4001
-// tokens, 28 / 4 heads of 128, 139 us, 5.7 TB/s; 64 x 750..1500, 32 / 8 heads, 34 us, 4.1 TB/s, of which 8 us pass until the first tiles are here.
+// tokens, 28 / 4 heads of 128, 140 us, 5.7 TB/s; 64 x 750..1500, 32 / 8 heads, 35 us, 4.0 TB/s, of which 8 us pass until the first tiles are here.
 //
 // Split: every (sequence, head) item is cut into units of U chunks of 64 tokens, U from the whole batch's tokens, whatever the lengths are.
 // Block i takes units i, i + grid, ...: about one each, so that taking them from a counter instead (SMs do not get equal shares of the

@@ -19,7 +19,7 @@
 //   (4) Where even those bins are too full (thousands of equal logits, a long top-k), the range is cut again, until one value is left.
 // Then the blocks sum their kept weights by index, and the one in whose share u * W falls looks for the token.
 //
-// Measured (one B200, 151936 logits, device time): 1 row top-k 19 us, 64 rows of nuclei 93 us, 256 rows of all kinds 168 us. Reading the logits
+// Measured (one B200, 151936 logits, device time): 1 row top-k 19 us, 64 rows of nuclei 94 us, of min-p 44 us, 256 rows of all kinds 170 us. Reading the logits
 // would take 0.1, 6 and 24 us: the time goes to a row's chain of steps (18 us for a usual row, 42 for a nucleus of tens of thousands), of which
 // 33 rows run at a time (two blocks on an SM, and whole clusters of eight in a GPC); inside them to issue slots, shared-memory atomics and the exchanges. (Read again
 // from the second-level cache instead, with clusters of four and twice the rows at a time, the same cases took 21, 99 and 178 us where this took 19, 99 and 181.)
